@@ -12,10 +12,14 @@
 //                TMEM).  The two have results and references of their own, like two pieces of a split unit, and add
 //                them up at its end; then q of the next unit is in shared memory already.
 //
-// Rounding: (code - 8) * scale has at most 11 significant bits, so in float16 it is exact; the scales of a tile
-// are divided by its largest one's power of two, which goes into the scores' factor, or, for V, into the weights'.
-// q is scaled by a power of two for each row, the weights are relative to a running reference: what is rounded is a
-// weight, to 11 bits, and the result.
+// Rounding: (code - 8) * scale has at most 11 significant bits, so in float16 it is exact; K's scales are divided by a
+// power of two for each tile, which goes into the scores' factor, V's by one that changes where a tile's scales are
+// larger or much smaller than those before (the results, in fp32, are multiplied by the difference).  q is scaled by a
+// power of two for each row.  The weights are float16 too, so they are held at a size of their own: for softmax the
+// largest so far is at 2^7 to 2^15; for SiLU 2^15 is what no score can reach, |alpha| D max |q| times the tile's largest
+// code and scale, which is 2^7 or so times the usual ones.  So no finite score overflows, and weights keep their 11 bits
+// down to 2^-21 of the largest (2^-29 of SiLU's bound).  What is rounded is a weight, to 11 bits, and the result;
+// tanh.approx, as in the attention over 16-bit keys, is off by 2^-11 of half the score.
 //
 // A score costs one operation of the special-function unit (16 a clock and SM), 128 x 128 of them 1024 clocks; the
 // tile's two products take 512 clocks at head dimension 128, the conversions about 500 issue slots of each
@@ -40,9 +44,9 @@ struct __align__(16) RingSlot {
   const uint8_t *codes[8];         // K codes of 16 positions; nullptr: none
   uint16_t scales[2][TC_TILE * 2]; // float16, K and V, [position][group]
   float k_factor;                  // 2^e that K's scales were divided by
+  int k_ref;                       // SiLU: the e, or a larger one, that the weights' size goes by
   int v_exp;                       // e of V's
   int flags;
-  int pad;
   uint32_t bad[4];                 // positions whose V is no number
 };
 
@@ -68,6 +72,22 @@ __device__ __forceinline__ uint4 eight_values(uint32_t x, uint32_t s1, uint32_t 
   r.w = half2_mul(k_exact(k_pair(x >> 8, true), true), s16);
   return r;
 }
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + min(max(e, -126), 127)) << 23); }
+__device__ __forceinline__ float pow2_far(int e) { return pow2(e / 2) * pow2(e - e / 2); }   // beyond fp32's normal numbers
+
+// A power of two that follows those of a unit's tiles, which it may be above by `above` and below by `below` at most;
+// otherwise it is set to one above by `set`.  Results are held relative to it, so it does not fall below its largest so
+// far by more than `fall`: 2^44 for V and 2^30 for K together leave results of 2^50 within fp32.
+struct Follow {
+  int at, most;
+  __device__ __forceinline__ void next(bool first, bool none, int e, int above, int below, int set, int fall) {
+    if (first) at = most = -126;
+    if (none) return;   // (all zeros: nothing to go by)
+    if (at - e > above || e - at > below) at = max(max(e + set, most - fall), -126);
+    most = max(most, at);
+  }
+};
+
 // column c of a row's eight holds value ..
 __device__ __forceinline__ constexpr int value_of(int c) { return (c >> 1) + 4 * (c & 1); }
 
@@ -113,7 +133,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
   volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(gen + SM::BARS + 304);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(gen + SM::BARS + 312);
   __shared__ RunSmem<TC_WARPS> s_run;
-  __shared__ float s_ml[2][TC_ROWS][2];
+  __shared__ float s_top[2][TC_ROWS], s_sum[2][TC_ROWS];
+  __shared__ int s_ref[2][TC_ROWS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const WaitCtx wc{abort_flag, a.status};
 
@@ -217,6 +238,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
     look_up(f[1]);
     step(f[1]);
     request(f[0], sc[0]);
+    Follow k_ref{0, 0}, v_ref{0, 0};
     auto hand_out = [&](uint32_t i, const Info &now, const uint4 (&scales)[2]) {
       RingSlot &slot = ring[i % RING_SLOTS];
       ok = mbar_wait(wc, ring_empty + 8 * (i % RING_SLOTS), ((i / RING_SLOTS) & 1) ^ 1, 961);
@@ -238,7 +260,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
           else if (kv == 1) bad |= 1u << x, s[x] = 0;
         }
         most = __reduce_max_sync(0xffffffffu, most);
-        const int e = most == 0 ? 0 : max((int)(most >> 7) - 127, -126);
+        int e = max((int)(most >> 7) - 127, -126);   // of the largest scale
+        if (kv == 0) {
+          k_ref.next(now.flags & TILE_FIRST, most == 0, e, 8, 0, 1, 30);
+        } else {
+          v_ref.next(now.flags & TILE_FIRST, most == 0, e, 3, 1, 0, 44);
+          e = v_ref.at;
+        }
         exps[kv] = e;
         const float down = __int_as_float((127 - e) << 23);
         uint32_t h[4];
@@ -259,7 +287,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
         }
       }
       if (lane == 0) {
-        slot.k_factor = __int_as_float((127 + exps[0]) << 23);
+        slot.k_factor = pow2(exps[0]);
+        slot.k_ref = k_ref.at;
         slot.v_exp = exps[1];
         slot.flags = now.flags | (any_bad ? TILE_BAD : 0);
       }
@@ -428,7 +457,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;             // (lane offset of the warp's quarter, bits 16 and up)
     const uint32_t ts = tmem + lanes + side * 128, to = tmem_o + lanes + side * 128;
     // q of a row as float16, scaled by a power of two to at most 1: of a pair each side has its own rows, otherwise each
-    // writes half of a row's values.  Returns the factor of the row's scores.
+    // writes half of a row's values.  Returns the factor of the row's scores; `bound`: they are below 2^bound times K's
+    // factor of the tile.
+    int bound = 0;
     auto load_q = [&]() {
       const SeqShape &seq = walk.seq;
       const bool pair = seq.rows - walk.rb * TC_BLOCK > TC_ROWS;
@@ -456,6 +487,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
           for (int y = 0; y < 8; ++y) most = fmaxf(most, fabsf(x[y]));
         }
       }
+      if (!SOFTMAX) bound = (__float_as_int(most * fabsf(a.alpha) * (1.01f * D * 7.f * 2.f)) >> 23) - 126;   // (1.01: q's rounding)
       const int e = min(max((__float_as_int(most) >> 23) - 126, -125), 125);
       const float down = __int_as_float((127 - e) << 23) * (a.alpha < 0.f ? -1.f : 1.f);
       uint8_t *tile = gen + SM::Q + (pair ? side * SM::TILE : 0) + r * 128;
@@ -487,7 +519,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
                                   : RowSees{0, 0, -1};
       }();
       float top = SOFTMAX ? -3.0e38f : 0.f, sum = 0.f;
-      int ref = 0;          // SiLU: the result so far is in units of 2^(ref - 4)
+      int ref = 0;          // the result so far is in units of 2^ref
       const uint32_t end = begin + here, before = count;
       const int first_pos = (walk.range.first_tile<TC_TILE>() + walk.tile) * TC_TILE;
       for (uint32_t i = begin; i < end && ok; ++i) {
@@ -501,7 +533,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
         ok = ok && mbar_wait(wc, s_full + 8 * side, count & 1, 971);
         if (!ok) break;
         tc_fence_after();
-        const float factor = fmaxf(mul * slot.k_factor, 1.2e-38f);   // (above 0: an unseen score stays -inf)
+        const float factor = SOFTMAX ? fmaxf(mul * slot.k_factor, 1.2e-38f) : mul * slot.k_factor;   // (above 0: an unseen score stays -inf)
         const int v_exp = slot.v_exp;
         const int pos0 = first_pos + (int)(i - begin) * TC_TILE;
         const bool bad = slot.flags & TILE_BAD;
@@ -542,7 +574,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
           }
           tc_wait_st();
         };
-        float p_factor = 1.f;
+        float p_factor = 1.f, shift = 0.f;
         if (SOFTMAX) {
           float m = -INFINITY;
 #pragma unroll 1
@@ -551,23 +583,25 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
 #pragma unroll
             for (int x = 0; x < 32; x += 2) m = fmaxf(m, fmaxf(__uint_as_float(s[x]), __uint_as_float(s[x + 1])));
           }
-          m = m * factor + (float)v_exp;
-          if (__any_sync(0xffffffffu, m > top + 8.f)) {   // (weights up to 2^8 do no harm)
-            m = fmaxf(m, top);
+          m *= factor;
+          const bool higher = __any_sync(0xffffffffu, m > top + 8.f);
+          if (higher || v_exp != ref) {
+            m = higher ? fmaxf(m, top) : top;
             const float by = ex2(top - m);
-            rescale(by);
+            rescale(by * pow2(ref - v_exp));
             sum *= by;
             top = m;
-          }
-        } else {
-          if (count == before) ref = v_exp;
-          if (v_exp > ref + 8) {
-            rescale(ex2((float)(ref - v_exp)));
             ref = v_exp;
           }
-          p_factor = ex2((float)(v_exp - ref + 4));
+          shift = 7.f - top;
+        } else {
+          const int t = min(max(15 - bound - slot.k_ref, -126), 126), now = v_exp - t;
+          if (__any_sync(0xffffffffu, now != ref)) {
+            rescale(pow2(ref - now));
+            ref = now;
+          }
+          p_factor = pow2(t);
         }
-        const float shift = SOFTMAX ? (float)v_exp - top : 0.f;
         float part0 = 0.f, part1 = 0.f;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
@@ -591,7 +625,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
           }
           tmem_st16(ts + 16 * c, p);
         }
-        if (SOFTMAX) sum += (part0 + part1) * ex2((float)-v_exp);
+        if (SOFTMAX) sum += part0 + part1;
         tc_wait_st();
         tc_fence_before();
         wait_sum();
@@ -605,8 +639,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
       // ---------------------------------------------------------- q of the next unit, then the result of this one
       const Walk<TC_BLOCK, TC_TILE> done = walk;
       if (count != before && ok) ok = mbar_wait(wc, pv_done + 8 * side, (count - 1) & 1, 974);
-      s_ml[side][r][0] = SOFTMAX ? top : (float)ref;
-      s_ml[side][r][1] = sum;
+      s_top[side][r] = top;
+      s_sum[side][r] = sum;
+      s_ref[side][r] = ref;
       tc_fence_before();
       if (rows_any(!ok)) break;        // (all eight warps or none: whoever gave up still comes here)
       tc_fence_after();
@@ -615,16 +650,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
       {
         const bool both = !pair && here > 1;   // (the side of a unit's only tile has it all)
         const int lead = pair ? side : begin & 1;
-        const float t0 = s_ml[lead][r][0], t1 = s_ml[lead ^ 1][r][0];
-        float f0, f1, m = 0.f, l = 0.f;
-        if (SOFTMAX) {
+        float f0 = pow2_far(s_ref[lead][r]), f1 = pow2_far(s_ref[lead ^ 1][r]), m = 0.f, l = 0.f;
+        if (SOFTMAX) {   // (weights of up to 2^15 are numbers of up to 1 from here on)
+          const float t0 = s_top[lead][r], t1 = s_top[lead ^ 1][r];
           m = both ? fmaxf(t0, t1) : t0;
-          f0 = ex2(t0 - m);
-          f1 = ex2(t1 - m);
-          l = s_ml[lead][r][1] * f0 + (both ? s_ml[lead ^ 1][r][1] * f1 : 0.f);
-        } else {
-          f0 = ex2(t0 - 4.f);
-          f1 = ex2(t1 - 4.f);
+          const float w0 = ex2(t0 - m) * 0x1p-15f, w1 = ex2(t1 - m) * 0x1p-15f;
+          l = s_sum[lead][r] * w0 + (both ? s_sum[lead ^ 1][r] * w1 : 0.f);
+          f0 *= w0;
+          f1 *= w1;
         }
         const bool whole = done.whole();
         const int at = done.rb * TC_BLOCK + (pair ? side * TC_ROWS : 0) + r;
@@ -667,7 +700,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
         }
       }
       tc_fence_before();
-      asm volatile("bar.sync 1, 256;" ::: "memory");   // (s_ml is free)
+      asm volatile("bar.sync 1, 256;" ::: "memory");   // (s_top, s_sum and s_ref are free)
       if (lane == 0) mbar_arrive(o_empty);
       if (threadIdx.x == 0) leave_join(a, done, total, G);
       begin = end;
