@@ -12,9 +12,12 @@
 //                TMEM).  The two have results and references of their own, like two pieces of a split unit, and add
 //                them up at its end; then q of the next unit is in shared memory already.
 //
-// Rounding: (code - 8) * scale has at most 11 significant bits, so in float16 it is exact; K's scales are divided by a
-// power of two for each tile, which goes into the scores' factor, V's by one that changes where a tile's scales are
-// larger or much smaller than those before (the results, in fp32, are multiplied by the difference).  q is scaled by a
+// Rounding: (code - 8) * scale has at most 11 significant bits, so in float16 it is exact for scales from 2^12 down to
+// 2^-13 (odd pairs of codes are 16 times too large and meet a sixteenth of the scale).  K's scales are divided by a power of two
+// for each tile that leaves the largest at 2^12, and goes into the scores' factor; V's by one that leaves it at 2^9 to
+// 2^12 and changes where a tile's scales leave that range (the results, in fp32, are multiplied by the difference).  So
+// scales down to 2^-25 and 2^-22 of a tile's largest are exact, whichever rows see that one and whichever group of 64
+// values it is in; smaller ones lose a bit for each power of two.  q is scaled by a
 // power of two for each row.  The weights are float16 too, so they are held at a size of their own: for softmax the
 // largest so far is at 2^7 to 2^15; for SiLU 2^15 is what no score can reach, |alpha| D max |q| times the tile's largest
 // code and scale, which is 2^7 or so times the usual ones.  So no finite score overflows, and weights keep their 11 bits
@@ -38,6 +41,7 @@ constexpr int TC_THREADS = 448, TC_WARPS = TC_THREADS / 32;
 constexpr int TC_ROWS = 128, TC_BLOCK = 2 * TC_ROWS, TC_TILE = 128;   // rows of a product, of a unit; positions of a tile
 constexpr int RING_SLOTS = 8;
 constexpr int RING_READERS = 13;  // 8 + 4 + 1 warps
+constexpr int SCALE_AT = 12;      // exponent of the largest scale that float16 has room for: 7 * 2^13 < 65504
 enum { TILE_FIRST = 1, TILE_PAIR = 2, TILE_BAD = 4 };
 
 struct __align__(16) RingSlot {
@@ -260,11 +264,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
           else if (kv == 1) bad |= 1u << x, s[x] = 0;
         }
         most = __reduce_max_sync(0xffffffffu, most);
-        int e = max((int)(most >> 7) - 127, -126);   // of the largest scale
+        int e = max((int)(most >> 7) - 127 - SCALE_AT, -126);
         if (kv == 0) {
           k_ref.next(now.flags & TILE_FIRST, most == 0, e, 8, 0, 1, 30);
         } else {
-          v_ref.next(now.flags & TILE_FIRST, most == 0, e, 3, 1, 0, 44);
+          v_ref.next(now.flags & TILE_FIRST, most == 0, e, 3, 0, 1, 44);
           e = v_ref.at;
         }
         exps[kv] = e;
@@ -487,7 +491,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
           for (int y = 0; y < 8; ++y) most = fmaxf(most, fabsf(x[y]));
         }
       }
-      if (!SOFTMAX) bound = (__float_as_int(most * fabsf(a.alpha) * (1.01f * D * 7.f * 2.f)) >> 23) - 126;   // (1.01: q's rounding)
+      if (!SOFTMAX) bound = (__float_as_int(most * fabsf(a.alpha) * (1.01f * D * 7.f * (2 << SCALE_AT))) >> 23) - 126;   // (1.01: q's rounding)
       const int e = min(max((__float_as_int(most) >> 23) - 126, -125), 125);
       const float down = __int_as_float((127 - e) << 23) * (a.alpha < 0.f ? -1.f : 1.f);
       uint8_t *tile = gen + SM::Q + (pair ? side * SM::TILE : 0) + r * 128;

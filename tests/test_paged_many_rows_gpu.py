@@ -160,3 +160,28 @@ def test_tiles_of_zeros_and_tiny_values(lengths, new, softmax):
     cache, table = make_cache(lengths, 1, 128, 64, v_exp=exp, seed=6)
     for window in (0, 60):
         check(cache, table, lengths, new, 2, torch.bfloat16, softmax, window=window)
+
+
+SPREAD = {
+    # exponents of the scales within a tile
+    "first group small": lambda b, pos, group: -20 * (group == 0) + 0 * pos,
+    "second group small": lambda b, pos, group: -20 * (group == 1) + 0 * pos,
+    "positions": lambda b, pos, group: -((pos * 7919 + b) % 21) + 0 * group,
+    "one large": lambda b, pos, group: 20 * (pos % 128 == 77) - 10 + 0 * group,
+    "groups and positions": lambda b, pos, group: -((pos * 31 + group * 11) % 21),
+}
+
+
+@pytest.mark.parametrize("spread", sorted(SPREAD))
+@pytest.mark.parametrize("softmax", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lengths,new", ROWS)
+def test_scales_far_apart_within_a_tile(lengths, new, dtype, softmax, spread):
+    """Up to 2^20 between the scales of a tile, in V and in K: of positions that a row need not see (a window of a few,
+    candidates that see none of each other) and of the groups, which are columns of their own."""
+    exp = SPREAD[spread]
+    targets = [n // 2 for n in new]
+    for k_exp, v_exp in ((None, exp), (exp, None)):
+        cache, table = make_cache(lengths, 2, 128, 64, k_exp, v_exp, seed=7)
+        for nt, window in ((None, 0), (None, 3), (targets, 0), (targets, 3)):
+            check(cache, table, lengths, new, 2, dtype, softmax, nt, window)
