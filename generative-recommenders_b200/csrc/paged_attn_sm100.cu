@@ -51,7 +51,7 @@ struct __align__(16) RingSlot {
   int k_ref;                       // SiLU: the e, or a larger one, that the weights' size goes by
   int v_exp;                       // e of V's
   int flags;
-  uint32_t bad[4];                 // positions whose V is no number
+  uint32_t bad[2][4];              // positions whose V is no number in a group of 64 values
 };
 
 template <int D>
@@ -139,6 +139,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
   __shared__ RunSmem<TC_WARPS> s_run;
   __shared__ float s_top[2][TC_ROWS], s_sum[2][TC_ROWS];
   __shared__ int s_ref[2][TC_ROWS];
+  __shared__ uint8_t s_lost[2][TC_ROWS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const WaitCtx wc{abort_flag, a.status};
 
@@ -281,13 +282,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
           *reinterpret_cast<uint4 *>(&slot.scales[kv][blk * PA_BLOCK * G64 + part * 8]) = make_uint4(h[0], h[1], h[2], h[3]);
       }
       const bool any_bad = __any_sync(0xffffffffu, bad != 0);
-      if (lane < 4) slot.bad[lane] = 0;
+      if (lane < 8) slot.bad[lane >> 2][lane & 3] = 0;
       __syncwarp();
       if (any_bad && bad != 0) {
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
           const int key = blk * PA_BLOCK + (part * 8 + x) / G64;
-          if ((bad >> x) & 1) atomicOr(&slot.bad[key >> 5], 1u << (key & 31));
+          if ((bad >> x) & 1) atomicOr(&slot.bad[x % G64][key >> 5], 1u << (key & 31));
         }
       }
       if (lane == 0) {
@@ -524,6 +525,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
       }();
       float top = SOFTMAX ? -3.0e38f : 0.f, sum = 0.f;
       int ref = 0;          // the result so far is in units of 2^ref
+      uint32_t lost = 0;    // groups of 64 values in which the row sees a V that is no number
       const uint32_t end = begin + here, before = count;
       const int first_pos = (walk.range.first_tile<TC_TILE>() + walk.tile) * TC_TILE;
       for (uint32_t i = begin; i < end && ok; ++i) {
@@ -540,22 +542,28 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
         const float factor = SOFTMAX ? fmaxf(mul * slot.k_factor, 1.2e-38f) : mul * slot.k_factor;   // (above 0: an unseen score stays -inf)
         const int v_exp = slot.v_exp;
         const int pos0 = first_pos + (int)(i - begin) * TC_TILE;
-        const bool bad = slot.flags & TILE_BAD;
-        const bool masked = bad || pos0 < walk.range.all_lo || pos0 + TC_TILE > walk.range.all_hi;
-        // scores of 32 columns; unseen ones to `none`, those of positions whose V is no number to NaN
+        const bool masked = pos0 < walk.range.all_lo || pos0 + TC_TILE > walk.range.all_hi;
+        auto seen_bits = [&](int c) {   // of 32 columns
+          const int at = pos0 + 32 * c;
+          return range_bits(sees.lo - at, sees.hi - at) | range_bits(sees.self - at, sees.self - at + 1);
+        };
+        if (slot.flags & TILE_BAD) {   // (those V are zeros in the product)
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+#pragma unroll
+            for (int g = 0; g < G64; ++g) lost |= (seen_bits(c) & slot.bad[g][c]) != 0 ? 1u << g : 0u;
+          }
+        }
+        // scores of 32 columns; unseen ones to `none`
         uint32_t s[32];
         auto load = [&](int c, float none) {
           tmem_ld32(ts + 32 * c, s);
           tc_wait_ld();
           if (masked) {
-            const int at = pos0 + 32 * c;
-            const uint32_t bits = range_bits(sees.lo - at, sees.hi - at) | range_bits(sees.self - at, sees.self - at + 1);
-            const uint32_t nan = bad ? slot.bad[c] : 0u;
+            const uint32_t bits = seen_bits(c);
 #pragma unroll
-            for (int x = 0; x < 32; ++x) {
+            for (int x = 0; x < 32; ++x)
               if (!((bits >> x) & 1)) s[x] = __float_as_uint(none);
-              else if ((nan >> x) & 1) s[x] = 0x7fffffffu;
-            }
           }
         };
         // this side's sum before: its end is waited for before the next can begin (a parity says which of two phases
@@ -646,6 +654,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
       s_top[side][r] = top;
       s_sum[side][r] = sum;
       s_ref[side][r] = ref;
+      s_lost[side][r] = (uint8_t)lost;
       tc_fence_before();
       if (rows_any(!ok)) break;        // (all eight warps or none: whoever gave up still comes here)
       tc_fence_after();
@@ -671,6 +680,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
         const float last = !whole ? 1.f : !SOFTMAX ? a.scale : l == 0.f ? 0.f : 1.f / l;
         f0 *= last;
         f1 *= last;
+        lost = s_lost[lead][r] | (both ? s_lost[lead ^ 1][r] : 0);
         T *out = static_cast<T *>(a.out) + ((int64_t)(done.seq.q_start + row_i) * a.Hq + hq) * D;
 #pragma unroll 1
         for (int c = pair ? 0 : side * (D / 32); c < (pair ? D / 16 : (side + 1) * (D / 32)); ++c) {   // 16 columns at a time
@@ -683,7 +693,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
             float x[8];
 #pragma unroll
             for (int y = 0; y < 8; ++y) {
-              x[value_of(y)] = __uint_as_float(o[8 * u + y]) * f0;
+              x[value_of(y)] = __uint_as_float(o[8 * u + y]) * ((lost >> (c / 4)) & 1 ? __int_as_float(0x7fffffff) : f0);
               if (both) x[value_of(y)] += __uint_as_float(o1[8 * u + y]) * f1;
             }
             if (on && whole) {
@@ -704,7 +714,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
         }
       }
       tc_fence_before();
-      asm volatile("bar.sync 1, 256;" ::: "memory");   // (s_top, s_sum and s_ref are free)
+      asm volatile("bar.sync 1, 256;" ::: "memory");   // (s_top, s_sum, s_ref and s_lost are free)
       if (lane == 0) mbar_arrive(o_empty);
       if (threadIdx.x == 0) leave_join(a, done, total, G);
       begin = end;

@@ -185,3 +185,46 @@ def test_scales_far_apart_within_a_tile(lengths, new, dtype, softmax, spread):
         cache, table = make_cache(lengths, 2, 128, 64, k_exp, v_exp, seed=7)
         for nt, window in ((None, 0), (None, 3), (targets, 0), (targets, 3)):
             check(cache, table, lengths, new, 2, dtype, softmax, nt, window)
+
+
+@pytest.mark.parametrize("softmax", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lengths,new", ROWS + [([300, 150, 40], [5, 2, 9])])
+def test_values_that_are_no_numbers(lengths, new, dtype, softmax):
+    """A group of V that is NaN makes that group's columns NaN of the rows that see it, and nothing else."""
+    cache, table = make_cache(lengths, 2, 128, 64, seed=8)
+    v = torch.randn(len(lengths), 2, 128, device=DEV)
+    v[0, 0, 3] = float("inf")        # head 0, first group, of position 250
+    v[1, 1, 100] = float("nan")      # head 1, second group, of position 140
+    v[2, 0, 5] = v[2, 0, 127] = float("nan")   # both, of the last position
+    at = torch.tensor([250, 140, lengths[2] - 1], device=DEV)
+    G.append_paged_kv(cache, v.nan_to_num(1.0, 1.0), v, table, at, offsets_of([1] * 3))
+    for targets, window in ((None, 0), (None, 20), ([n // 2 for n in new], 0)):
+        check(cache, table, lengths, new, 4, dtype, softmax, targets, window)
+
+
+@pytest.mark.parametrize("softmax", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [40, 140])
+def test_positions_without_a_page(rows, dtype, softmax):
+    """Rows that see a position past the table or on a page that is none are NaN, the others as ever."""
+    lengths = [300, 270, 150]
+    cache, table = make_cache(lengths, 2, 64, 16, seed=2)
+    bad = table.clone()
+    bad[0, 12] = -1                       # positions 192 ..
+    bad[1, 16] = cache.num_pages + 5      # 256 ..
+    q = torch.randn(3 * rows, 4, 64, generator=torch.Generator().manual_seed(1)).to(dtype).to(DEV)
+    most = 16 * table.shape[1]
+    for window in (0, 30):
+        good, out = (G.paged_mha(512, 0.1, q, cache, t, torch.tensor(n, device=DEV), offsets_of([rows] * 3),
+                                 max_attn_len=window, activation="softmax" if softmax else "silu").view(3, rows, 4, 64)
+                     for t, n in ((table, lengths), (bad, [300, 270, most + 3])))
+        nan = torch.isnan(out).flatten(2)
+        assert torch.equal(nan.any(2), nan.all(2))
+        pos = torch.tensor([300, 270, most + 3])[:, None] - rows + torch.arange(rows)
+        start = (pos - window).clamp(min=0) if window else torch.zeros_like(pos)
+        first, last = torch.tensor([[192, 208], [256, 272], [150, 1000]]).unbind(1)   # (from 150 on: never written, ones)
+        assert torch.equal(nan.all(2).cpu(), (pos >= first[:, None]) & (start < last[:, None]))
+        same = ~nan.all(2)
+        same[2] = False
+        assert float((out[same].double() - good[same].double()).norm()) <= 2 * UNIT[dtype] * float(good[same].double().norm())
