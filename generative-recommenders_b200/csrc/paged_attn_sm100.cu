@@ -41,7 +41,7 @@ constexpr int TC_THREADS = 448, TC_WARPS = TC_THREADS / 32;
 constexpr int TC_ROWS = 128, TC_BLOCK = 2 * TC_ROWS, TC_TILE = 128;   // rows of a product, of a unit; positions of a tile
 constexpr int RING_SLOTS = 8;
 constexpr int RING_READERS = 13;  // 8 + 4 + 1 warps
-constexpr int SCALE_AT = 12;      // exponent of the largest scale that float16 has room for: 7 * 2^13 < 65504
+constexpr int SCALE_AT = 12;      // exponent of the largest scale that float16 has room for, code 0 too: 8 * 255 / 128 * 2^12 < 65504
 enum { TILE_FIRST = 1, TILE_PAIR = 2, TILE_BAD = 4 };
 
 struct __align__(16) RingSlot {
@@ -261,7 +261,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
         for (int x = 0; x < 8; ++x) {
           const int pos = now.pos + blk * PA_BLOCK + (part * 8 + x) / G64;
           if (pos < now.begin || pos >= now.end) s[x] = 0;
-          if (s[x] < 0x7f80u) most = max(most, (uint32_t)s[x]);   // (scales are not negative; a sign bit is no number either)
+          const uint32_t size = s[x] & 0x7fffu;   // (append makes no negative scales, but they are numbers)
+          if (size < 0x7f80u) most = max(most, size);
           else if (kv == 1) bad |= 1u << x, s[x] = 0;
         }
         most = __reduce_max_sync(0xffffffffu, most);
@@ -492,7 +493,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
           for (int y = 0; y < 8; ++y) most = fmaxf(most, fabsf(x[y]));
         }
       }
-      if (!SOFTMAX) bound = (__float_as_int(most * fabsf(a.alpha) * (1.01f * D * 7.f * (2 << SCALE_AT))) >> 23) - 126;   // (1.01: q's rounding)
+      if (!SOFTMAX) bound = (__float_as_int(most * fabsf(a.alpha) * (1.01f * D * 8.f * (2 << SCALE_AT))) >> 23) - 126;   // (1.01: q's rounding)
       const int e = min(max((__float_as_int(most) >> 23) - 126, -125), 125);
       const float down = __int_as_float((127 - e) << 23) * (a.alpha < 0.f ? -1.f : 1.f);
       uint8_t *tile = gen + SM::Q + (pair ? side * SM::TILE : 0) + r * 128;

@@ -25,8 +25,9 @@ UNIT = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}    # one rounding 
 SMALL = {torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -25}  # and below the normal numbers
 
 
-def make_cache(lengths, H, d, page, k_exp=None, v_exp=None, seed=0):
-    """Random codes; scales of 0.2 to 0.5 times 2^exp, ``exp(b, position, group)`` whole numbers that broadcast."""
+def make_cache(lengths, H, d, page, k_exp=None, v_exp=None, seed=0, signs=False):
+    """Random codes; scales of 0.2 to 0.5 (with ``signs`` -0.2 to -0.5 as well, and code 0) times 2^exp, ``exp(b, position, group)``
+    whole numbers that broadcast."""
     g = torch.Generator().manual_seed(seed)
     need = [-(-n // page) for n in lengths]
     order = torch.randperm(sum(need) + 2, generator=g)
@@ -42,9 +43,11 @@ def make_cache(lengths, H, d, page, k_exp=None, v_exp=None, seed=0):
             m = min(page, n - i * page)
             pos = torch.arange(i * page, i * page + m)[:, None]
             for kv, exp in enumerate((k_exp, v_exp)):
-                x = torch.randint(1, 16, (H, m, d), generator=g)
+                x = torch.randint(0 if signs else 1, 16, (H, m, d), generator=g)
                 pool[p, :, kv * codes:kv * codes + m * d // 2] = (x[..., 0::2] | x[..., 1::2] << 4).to(torch.uint8).flatten(1)
                 s = torch.rand(H, m, groups, generator=g, dtype=torch.float64) * 0.3 + 0.2
+                if signs:
+                    s = s * (torch.randint(0, 2, s.shape, generator=g) * 2 - 1)
                 if exp is not None:
                     s = s * 2.0 ** exp(b, pos, torch.arange(groups)[None]).double()
                 raw = s.bfloat16().flatten(1).contiguous().view(torch.uint8)
@@ -228,3 +231,16 @@ def test_positions_without_a_page(rows, dtype, softmax):
         same = ~nan.all(2)
         same[2] = False
         assert float((out[same].double() - good[same].double()).norm()) <= 2 * UNIT[dtype] * float(good[same].double().norm())
+
+
+@pytest.mark.parametrize("softmax", [False, True])
+@pytest.mark.parametrize("lengths,new", ROWS + [([300, 150, 40], [5, 2, 9])])
+def test_negative_scales(lengths, new, softmax):
+    """A cache that another program has filled: a scale is any finite bfloat16, a code any of 16."""
+    for d in (64, 128):
+        cache, table = make_cache(lengths, 2, d, 64, seed=9, signs=True)
+        check(cache, table, lengths, new, 4, torch.bfloat16, softmax)
+        top = cache.pages.clone()
+        at, groups = 64 * d, d // 64      # (of a head of a page: codes, then scales)
+        top[..., at:] = torch.tensor([0x7f, 0x3f], dtype=torch.uint8, device=DEV).repeat(2 * 64 * groups)   # 0.99609375
+        check(G.PagedKVCache(top, 64, d), table, lengths, new, 4, torch.float16, softmax)
