@@ -15,6 +15,8 @@ struct PagedCache {
   int page_shift;                 // log2 of the positions of a page
 
   __host__ __device__ __forceinline__ int page_size() const { return 1 << page_shift; }
+  // positions that a sequence can have pages for
+  __device__ __forceinline__ int positions() const { return (int)min((int64_t)width << page_shift, (int64_t)0x7ffffc00); }
   __host__ __device__ __forceinline__ int code_bytes() const { return d >> 1; }                    // of a row
   __host__ __device__ __forceinline__ int scale_bytes() const { return 2 * (d / PAGED_GROUP); }    // of a row
   __host__ __device__ __forceinline__ int64_t page_bytes() const {
@@ -41,6 +43,7 @@ struct PagedCache {
 struct RowSees {
   int lo, hi, self;   // self = -1: a row before the sequence's start, which sees nothing
   __host__ __device__ __forceinline__ bool operator()(int j) const { return (j >= lo && j < hi) || j == self; }
+  __host__ __device__ __forceinline__ bool past(int end) const { return (hi > lo && hi > end) || self >= end; }
 };
 __host__ __device__ __forceinline__ RowSees row_sees(int p, int len, int num_targets, int c, int W) {
   RowSees r{0, 0, p};

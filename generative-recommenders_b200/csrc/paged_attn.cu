@@ -572,7 +572,9 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_kernel(PagedAttn a) {
     float *pml = a.part_ml + ((int64_t)blockIdx.x * 2 + slot) * RB * 2;
     for (int x = tid; x < nrows * (D / 4); x += PA_THREADS) {
       const int r = x / (D / 4), e = x % (D / 4) * 4;
-      float m = -3.0e38f, l = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+      const RowSees sees = ONE ? one : RowSees{s_sees[r][0], s_sees[r][1], s_sees[r][2]};
+      const float none = sees.past(a.cache.positions()) ? __int_as_float(0x7fffffff) : 0.f;
+      float m = -3.0e38f, l = 0.f, v[4] = {none, none, none, none};
       if (SOFTMAX) {
 #pragma unroll
         for (int w = 0; w < PA_WARPS; ++w) m = fmaxf(m, s_ml[w][r][0]);

@@ -29,7 +29,8 @@ struct PagedAttn {
 // units of work
 // ---------------------------------------------------------------------------------------
 // What block `rb` of the new rows (times query heads of a cache head) of sequence b has to read: positions
-// [begin, end), that is [lo, hi) in multiples of 16; positions in [all_lo, all_hi) are seen by every row.
+// [begin, end), that is [lo, hi) in multiples of 16; positions in [all_lo, all_hi) are seen by every row.  Positions past
+// the table are left out, however long a sequence says it is: rows that see any are NaN (RowSees::past).
 struct UnitRange {
   int lo, hi, all_lo, all_hi, begin, end;
   template <int TILE> __device__ __forceinline__ int first_tile() const { return lo / TILE; }
@@ -54,7 +55,8 @@ __device__ __forceinline__ UnitRange unit_range(const PagedAttn &a, const SeqSha
   UnitRange r{0, PA_BLOCK, 0, 0, 0, 0};
   if (p1 < 0) return r;   // nothing visible: one block, all of it masked
   const RowSees lo = row_sees(max(p0, 0), s.len, s.targets, a.c, a.W), hi = row_sees(p1, s.len, s.targets, a.c, a.W);
-  const int end = max(max(lo.hi, hi.hi), p1 + 1);
+  const int end = min(max(max(lo.hi, hi.hi), p1 + 1), a.cache.positions());
+  if (lo.lo >= end) return r;
   r.begin = lo.lo;
   r.end = end;
   r.lo = lo.lo / PA_BLOCK * PA_BLOCK;
@@ -63,6 +65,7 @@ __device__ __forceinline__ UnitRange unit_range(const PagedAttn &a, const SeqSha
   // (a row that is no candidate sees itself right behind the rest)
   r.all_hi = min(lo.hi + (lo.hi == lo.self), hi.hi + (hi.hi == hi.self));
   if (p0 < a.c) r.all_hi = p0 < 0 ? 0 : min(r.all_hi, a.c + 1);
+  r.all_hi = min(r.all_hi, end);
   return r;
 }
 template <int RB>

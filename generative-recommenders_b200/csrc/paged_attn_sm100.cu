@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
       }();
       float top = SOFTMAX ? -3.0e38f : 0.f, sum = 0.f;
       int ref = 0;          // the result so far is in units of 2^ref
-      uint32_t lost = 0;    // groups of 64 values in which the row sees a V that is no number
+      uint32_t lost = sees.past(a.cache.positions()) ? 3 : 0;   // groups of 64 values in which the row sees a V that is no number
       const uint32_t end = begin + here, before = count;
       const int first_pos = (walk.range.first_tile<TC_TILE>() + walk.tile) * TC_TILE;
       for (uint32_t i = begin; i < end && ok; ++i) {

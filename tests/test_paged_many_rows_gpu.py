@@ -244,3 +244,25 @@ def test_negative_scales(lengths, new, softmax):
         at, groups = 64 * d, d // 64      # (of a head of a page: codes, then scales)
         top[..., at:] = torch.tensor([0x7f, 0x3f], dtype=torch.uint8, device=DEV).repeat(2 * 64 * groups)   # 0.99609375
         check(G.PagedKVCache(top, 64, d), table, lengths, new, 4, torch.float16, softmax)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [1, 12, 40, 300])
+@pytest.mark.parametrize("length", [1025, 10 ** 6 + 1, 2 ** 31 - 1])
+def test_lengths_far_past_the_table(length, rows, dtype):
+    """What is past the table costs nothing: the rows that see some of it are NaN, without a walk to a length that no
+    cache has."""
+    lengths = [1000, 1000, 700]
+    cache, table = make_cache(lengths, 2, 64, 64, seed=4)
+    q = torch.randn(3 * rows, 4, 64, generator=torch.Generator().manual_seed(2)).to(dtype).to(DEV)
+    for act in ("silu", "softmax"):
+        good, out = (G.paged_mha(1024, 0.1, q, cache, table, torch.tensor(n, device=DEV), offsets_of([rows] * 3),
+                                 activation=act).double().view(3, rows, 4, 64) for n in (lengths, [1000, length, 700]))
+        first = max(0, 1024 - length + rows)   # rows of the second sequence before the table's end see what they saw
+        assert torch.isnan(out[1, first:]).all()
+        for b in (0, 2):
+            assert float((out[b] - good[b]).norm()) <= 2 * UNIT.get(dtype, 1e-5) * float(good[b].norm())
+    # a table of no pages at all
+    none = torch.zeros(1, 0, dtype=torch.int32, device=DEV)
+    x = G.paged_mha(1024, 0.1, q[:rows], cache, none, torch.tensor([length], device=DEV), offsets_of([rows]))
+    assert torch.isnan(x).all()
