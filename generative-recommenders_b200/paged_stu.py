@@ -27,6 +27,15 @@ class RotarySTULayerConfig(STULayerConfig):
     rotary_base: float = 10000.0
 
 
+def _new_positions(cached_lengths: torch.Tensor, new_offsets: torch.Tensor, rows: int) -> torch.Tensor:
+    """The position of every new row; of rows that no sequence has (padding) any number."""
+    row = torch.arange(rows, device=new_offsets.device)
+    # (-1 before the first offset and B past the last: both are the entry that is added at the end)
+    seq = torch.searchsorted(new_offsets, row.to(new_offsets.dtype), right=True) - 1
+    first = torch.nn.functional.pad(cached_lengths - new_offsets[:-1].to(cached_lengths.dtype), (0, 1))
+    return first[seq] + row.to(cached_lengths.dtype)
+
+
 class RotarySTULayer(STULayer):
     """``STULayer`` with weights for the norms of q and k (``_q_norm_weight``, ``_k_norm_weight``, one entry per
     value of a head) and rotated positions; ``attention_dim`` and ``hidden_dim`` are the same."""
@@ -111,13 +120,12 @@ class RotarySTULayer(STULayer):
 
         ``page_table`` names pages for all of them.  ``max_seq_len`` is what divides SiLU's weights, the one that
         the layer was trained with.  Candidates (``num_targets``) that are not to stay are overwritten by the next
-        call when it is given the same ``cached_lengths``."""
+        call when it is given the same ``cached_lengths``.  Rows past ``new_offsets[-1]`` (padding) are in no sequence:
+        nothing is cached for them and their attention is zeros."""
         H, d = self._num_heads, self._attention_dim
         u, q, k, v = self._uqvk(new_x)
         lengths = cached_lengths + (new_offsets[1:] - new_offsets[:-1]).to(cached_lengths.dtype)
-        rows = torch.arange(new_x.shape[0], device=new_x.device)
-        seq = torch.searchsorted(new_offsets, rows.to(new_offsets.dtype), right=True) - 1
-        positions = (cached_lengths - new_offsets[:-1].to(cached_lengths.dtype))[seq] + rows.to(cached_lengths.dtype)
+        positions = _new_positions(cached_lengths, new_offsets, new_x.shape[0])
         with span("## qk_norm_rotary ##"):
             q, _ = qk_norm_rotary(q.view(-1, H, d), None, positions, self._cos, self._sin, self._q_norm_weight)
         with span("## append_paged_kv ##"):

@@ -1,0 +1,62 @@
+"""Serving from the paged cache as batches come: padding rows, sequences without rows, what the operators refuse."""
+
+import pytest
+import torch
+
+import generative_recommenders_b200 as G
+from generative_recommenders_b200 import paged_stu
+
+DEV = "cuda:0"
+
+
+def offsets_of(counts, device=DEV):
+    return torch.tensor([0] + list(counts)).cumsum(0).to(device)
+
+
+@pytest.mark.parametrize("length_type", [torch.int32, torch.int64])
+@pytest.mark.parametrize("offset_type", [torch.int32, torch.int64])
+def test_positions_of_new_rows(length_type, offset_type):
+    for cached, new, rows in (([5, 0, 7], [2, 0, 4], 6), ([5, 0, 7], [2, 0, 4], 9), ([3], [0], 2), ([], [], 3), ([9], [1], 1)):
+        pos = paged_stu._new_positions(torch.tensor(cached, dtype=length_type), offsets_of(new, "cpu").to(offset_type), rows)
+        want = [c + i for c, n in zip(cached, new) for i in range(n)]
+        assert pos.dtype == length_type and pos.shape == (rows,) and pos[:len(want)].tolist() == want
+
+
+def layer_of(dtype, **options):
+    torch.manual_seed(3)
+    layer = G.RotarySTULayer(G.RotarySTULayerConfig(embedding_dim=96, num_heads=2, hidden_dim=64, attention_dim=64,
+                                                    output_dropout_ratio=0.0, max_positions=400, **options))
+    return layer.to(DEV).to(dtype).eval()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("new,padding", [([3, 0, 1], 4), ([40, 20, 0], 130), ([0, 0, 0], 5)])
+def test_padding_rows(new, padding, dtype):
+    """Rows past the last offset are in no sequence: the others and the cache are what they are without them."""
+    layer = layer_of(dtype)
+    cached = torch.tensor([30, 0, 64], device=DEV)
+    table = torch.arange(21, dtype=torch.int32, device=DEV).view(3, 7)
+    rows = sum(new)
+    x = torch.randn(rows + padding, 96, device=DEV).to(dtype)
+    caches = [G.PagedKVCache(torch.zeros(21, 2, G.PagedKVCache.page_bytes(16, 64), dtype=torch.uint8, device=DEV), 16, 64)
+              for _ in range(2)]
+    outs = [layer.paged_forward(y, c, table, cached, offsets_of(new), 200) for y, c in zip((x[:rows], x), caches)]
+    assert torch.equal(caches[0].pages, caches[1].pages)
+    assert outs[1].shape == x.shape and torch.isfinite(outs[1]).all()
+    if rows:
+        # (where sums are cut depends on the number of rows)
+        assert float((outs[1][:rows] - outs[0]).float().norm()) <= (1e-2 if dtype == torch.bfloat16 else 1e-4) * float(outs[0].float().norm())
+    u = layer._uqvk(x)[0]
+    alone = layer._output(torch.zeros(rows + padding, 2, 64, device=DEV, dtype=dtype), u, x)
+    assert torch.equal(outs[1][rows:], alone[rows:])
+
+
+@pytest.mark.gpu
+def test_a_batch_of_no_sequences():
+    layer = layer_of(torch.bfloat16)
+    cache = layer.new_cache(2, 16)
+    none = torch.zeros(0, dtype=torch.long, device=DEV)
+    x = torch.randn(3, 96, device=DEV).bfloat16()
+    out = layer.paged_forward(x, cache, torch.zeros(0, 0, dtype=torch.int32, device=DEV), none, torch.zeros(1, dtype=torch.long, device=DEV), 64)
+    assert out.shape == x.shape and torch.isfinite(out).all()
