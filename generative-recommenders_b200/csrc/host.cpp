@@ -751,6 +751,7 @@ void check_pages(const Tensor &pages, int64_t page_size, int64_t d) {
   TORCH_CHECK(pages.is_cuda(), "tensors must live on a CUDA device; this library has no CPU path (pages)");
   TORCH_CHECK_TYPE(pages.scalar_type() == at::kByte, "pages must be uint8");
   TORCH_CHECK(pages.dim() == 3 && pages.is_contiguous(), "pages must be a contiguous [pages, heads, bytes]");
+  TORCH_CHECK(pages.size(1) > 0, "a cache of no heads");
   TORCH_CHECK(pages.size(2) == 2 * page_size * (d / 2 + 2 * (d / 64)), "a page of ", page_size, " positions of ", d,
               " values has ", 2 * page_size * (d / 2 + 2 * (d / 64)), " bytes for a head, not ", pages.size(2));
 }

@@ -60,3 +60,9 @@ def test_a_batch_of_no_sequences():
     x = torch.randn(3, 96, device=DEV).bfloat16()
     out = layer.paged_forward(x, cache, torch.zeros(0, 0, dtype=torch.int32, device=DEV), none, torch.zeros(1, dtype=torch.long, device=DEV), 64)
     assert out.shape == x.shape and torch.isfinite(out).all()
+
+
+@pytest.mark.gpu
+def test_a_cache_of_no_heads_is_refused():
+    with pytest.raises(RuntimeError, match="no heads"):
+        G.PagedKVCache.allocate(4, 0, 64, 16)
