@@ -758,6 +758,7 @@ void check_pages(const Tensor &pages, int64_t page_size, int64_t d) {
 
 Tensor fill_cache(b200_hstu_paged_cache &c, const Tensor &pages, int64_t page_size, int64_t d, const Tensor &table_,
                   const Tensor &first) {
+  check_pages(pages, page_size, d);   // (a cache's fields may have changed since it was made)
   on_device_of(pages, first, "the cache");
   on_device_of(table_, first, "page_table");
   TORCH_CHECK_TYPE(table_.scalar_type() == at::kInt, "page_table must be int32");
@@ -780,12 +781,12 @@ void paged_append(const Tensor &pages, int64_t page_size, int64_t d, const Tenso
                   const MaybeTensor &sin, bool interleaved, const MaybeTensor &kw, double eps) {
   TORCH_CHECK(k_.is_cuda(), "tensors must live on a CUDA device; this library has no CPU path (k)");
   TORCH_CHECK(k_.dim() == 3 && v_.dim() == 3, "k and v must be 3-D");
+  b200_hstu_paged_append_args a = {};
+  const Tensor table = fill_cache(a.cache, pages, page_size, d, table_, k_);
   TORCH_CHECK(k_.sizes() == v_.sizes() && k_.size(1) == pages.size(1) && k_.size(2) == d, "k and v must be [rows, ",
               pages.size(1), ", ", d, "] like the cache");
   on_device_of(v_, k_, "v");
   TORCH_CHECK_TYPE(k_.scalar_type() == v_.scalar_type(), "k and v must share a dtype");
-  b200_hstu_paged_append_args a = {};
-  const Tensor table = fill_cache(a.cache, pages, page_size, d, table_, k_);
   const Tensor k = unit_stride(k_), v = unit_stride(v_);
   const Tensor cached = index_tensor(cached_, k, "cached_lengths", a.cache.B, B200_HSTU_LENGTHS_I64, a.index_flags);
   const Tensor offsets = index_tensor(offsets_, k, "new_offsets", a.cache.B + 1, B200_HSTU_OFFSETS_I64, a.index_flags);
@@ -838,10 +839,10 @@ Tensor paged_attention(const Tensor &q_, const Tensor &pages, int64_t page_size,
                        double scale, int64_t max_attn_len, int64_t contextual_seq_len, bool softmax, bool status) {
   TORCH_CHECK(q_.is_cuda(), "tensors must live on a CUDA device; this library has no CPU path (q)");
   TORCH_CHECK(q_.dim() == 3 && q_.size(2) == d, "q must be [rows, heads, ", d, "] like the cache");
-  TORCH_CHECK(q_.size(1) > 0 && q_.size(1) % pages.size(1) == 0, q_.size(1), " query heads on ", pages.size(1),
-              " heads of the cache");
   b200_hstu_paged_attn_args a = {};
   const Tensor table = fill_cache(a.cache, pages, page_size, d, table_, q_);
+  TORCH_CHECK(q_.size(1) > 0 && q_.size(1) % pages.size(1) == 0, q_.size(1), " query heads on ", pages.size(1),
+              " heads of the cache");
   const Tensor q = unit_stride(q_);
   const Tensor lengths = index_tensor(lengths_, q, "seq_lengths", a.cache.B, B200_HSTU_LENGTHS_I64, a.index_flags);
   const Tensor offsets = index_tensor(offsets_, q, "q_offsets", a.cache.B + 1, B200_HSTU_OFFSETS_I64, a.index_flags);

@@ -66,3 +66,21 @@ def test_a_batch_of_no_sequences():
 def test_a_cache_of_no_heads_is_refused():
     with pytest.raises(RuntimeError, match="no heads"):
         G.PagedKVCache.allocate(4, 0, 64, 16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("field,value", [("page_size", 32), ("head_dim", 128), ("pages", torch.zeros(4, 2, 100, dtype=torch.uint8)),
+                                         ("pages", torch.zeros(4, 2, 1088, dtype=torch.int8)), ("pages", torch.zeros(4, 1088, dtype=torch.uint8))])
+def test_fields_that_do_not_fit_any_more(field, value):
+    """A cache's fields can be replaced; every call looks at them before it hands them on."""
+    cache = G.PagedKVCache.allocate(4, 2, 64, 16)
+    setattr(cache, field, value.to(DEV) if isinstance(value, torch.Tensor) else value)
+    d = cache.head_dim
+    table = torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    one, x = torch.ones(1, dtype=torch.long, device=DEV), torch.zeros(1, 2, d, device=DEV)
+    with pytest.raises((RuntimeError, TypeError)):
+        G.append_paged_kv(cache, x, x, table, one, offsets_of([1]))
+    with pytest.raises((RuntimeError, TypeError)):
+        G.read_paged_kv(cache, table, offsets_of([1]), 1)
+    with pytest.raises((RuntimeError, TypeError)):
+        G.paged_mha(16, 1.0, x, cache, table, one, offsets_of([1]))
