@@ -845,6 +845,8 @@ int paged_attn_fwd(const b200_hstu_paged_attn_args &p, cudaStream_t st) {
   if (p.rows == 0) return 0;
   if (!p.q || !p.out || !p.q_offsets || (p.cache.B > 0 && !p.seq_lengths))
     return fail(B200_HSTU_EINVAL, "paged_attn: null tensor");
+  if ((((uintptr_t)p.out | (uintptr_t)p.workspace) & 15) != 0)
+    return fail(B200_HSTU_EINVAL, "paged_attn: out and workspace must be 16-byte aligned");
   a.q = p.q;
   a.out = p.out;
   a.lengths = {p.seq_lengths, (p.index_flags & B200_HSTU_LENGTHS_I64) ? 2 : 1};

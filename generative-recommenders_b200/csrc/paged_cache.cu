@@ -338,6 +338,7 @@ int paged_read(const b200_hstu_paged_read_args &p, cudaStream_t st) {
   if (p.rows < 0 || p.rows >= (1ll << 31)) return fail(B200_HSTU_EINVAL, "paged_read: bad number of rows");
   if (p.rows == 0) return 0;
   if (!p.k || !p.v || !p.seq_offsets) return fail(B200_HSTU_EINVAL, "paged_read: null tensor");
+  if ((((uintptr_t)p.k | (uintptr_t)p.v) & 15) != 0) return fail(B200_HSTU_EINVAL, "paged_read: k and v must be 16-byte aligned");
   a.out[0] = p.k, a.out[1] = p.v;
   a.offsets = {p.seq_offsets, (p.index_flags & B200_HSTU_OFFSETS_I64) ? 2 : 1};
   a.rows = p.rows;

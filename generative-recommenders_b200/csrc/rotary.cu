@@ -377,6 +377,8 @@ int norm_rotary(const b200_hstu_norm_rotary_args &p, bool bwd, cudaStream_t st) 
       return fail(B200_HSTU_EINVAL, "norm_rotary: weights must be float32 or of the activations' type");
     if (p.H[i] > 0 && p.rows > 0 && (!p.x[i] || (bwd ? !p.dy[i] || !p.dx[i] : !p.y[i])))
       return fail(B200_HSTU_EINVAL, "norm_rotary: null tensor");
+    if (p.H[i] > 0 && p.rows > 0 && ((uintptr_t)(bwd ? p.dx[i] : p.y[i]) & 15) != 0)
+      return fail(B200_HSTU_EINVAL, "norm_rotary: results must be 16-byte aligned");
     if (bwd && a.w[i] && !p.dweight[i]) return fail(B200_HSTU_EINVAL, "norm_rotary: null tensor");
   }
   if (p.H[0] + p.H[1] == 0) return 0;

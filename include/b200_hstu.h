@@ -362,7 +362,7 @@ int b200_hstu_append_kv(const b200_hstu_append_kv_args *args, b200_hstu_stream_t
  * pass:  y = R(pos) (x * rstd * w),  rstd = 1 / sqrt(mean(x^2) + eps),  where R turns every pair (a, b) of the
  * first `rotary` values into (a cos - b sin, b cos + a sin) with row `pos` of the tables; the pairs are
  * (i, i + rotary / 2), or (2i, 2i + 1) with `interleaved`.  x [rows, H, d] has unit stride on d; results are
- * contiguous.  Entry 0 of a pair of fields is q's, entry 1 k's; H = 0 leaves a tensor out, a NULL weight its
+ * contiguous and 16-byte aligned.  Entry 0 of a pair of fields is q's, entry 1 k's; H = 0 leaves a tensor out, a NULL weight its
  * norm, NULL positions the rotation.  A position outside the tables gives a row of NaN.
  *
  * The backward reads x and dy and writes dx and the weights' gradients (fp32, sums of fp32 partial sums that
@@ -432,7 +432,7 @@ int b200_hstu_paged_append(const b200_hstu_paged_append_args *args, b200_hstu_st
 
 /*
  * The values that the first seq_offsets[b + 1] - seq_offsets[b] positions of every sequence stand for: k, v
- * [rows, H, d], contiguous.  Rows without a page of the pool are NaN, rows beyond seq_offsets[B] zeros.
+ * [rows, H, d], contiguous and 16-byte aligned.  Rows without a page of the pool are NaN, rows beyond seq_offsets[B] zeros.
  */
 typedef struct b200_hstu_paged_read_args {
   b200_hstu_paged_cache cache;
@@ -459,7 +459,7 @@ int b200_hstu_paged_read(const b200_hstu_paged_read_args *args, b200_hstu_stream
 typedef struct b200_hstu_paged_attn_args {
   b200_hstu_paged_cache cache;
   const void *q;
-  void *out;                    /* [rows, Hq, d], contiguous */
+  void *out;                    /* [rows, Hq, d], contiguous, 16-byte aligned (workspace too) */
   const int32_t *seq_lengths;   /* [B] */
   const int32_t *q_offsets;     /* [B + 1] */
   const int32_t *num_targets;   /* [B] or NULL */
