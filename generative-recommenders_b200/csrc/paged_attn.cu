@@ -813,7 +813,7 @@ int launch_dim(PagedAttn &a, bool softmax, int nt, int grid, cudaStream_t st) {
 }
 
 bool sizes_ok(const b200_hstu_paged_attn_args &p) {
-  return p.rows >= 0 && p.Hq > 0 && p.cache.H > 0 && p.Hq % p.cache.H == 0 && p.cache.d > 0 && p.cache.B >= 0 &&
+  return p.rows >= 0 && p.rows < (1ll << 31) && p.Hq > 0 && p.cache.H > 0 && p.Hq % p.cache.H == 0 && p.cache.d > 0 && p.cache.B >= 0 &&
          p.rows * (int64_t)p.Hq < (1ll << 31) && p.cache.table_width >= 0;
 }
 
@@ -835,7 +835,7 @@ int paged_attn_status(const b200_hstu_paged_attn_args &p, cudaStream_t st, int32
 int paged_attn_fwd(const b200_hstu_paged_attn_args &p, cudaStream_t st) {
   PagedAttn a = {};
   if (int rc = check_paged_cache("paged_attn", p.cache, a.cache)) return rc;
-  if (p.rows < 0 || p.rows * (int64_t)p.Hq >= (1ll << 31)) return fail(B200_HSTU_EINVAL, "paged_attn: bad number of rows");
+  if (p.rows < 0 || p.rows >= (1ll << 31) || p.rows * (int64_t)p.Hq >= (1ll << 31)) return fail(B200_HSTU_EINVAL, "paged_attn: bad number of rows");
   if (p.Hq <= 0 || p.Hq % p.cache.H != 0)
     return fail(B200_HSTU_EINVAL, "paged_attn: %d query heads on %d heads of the cache", p.Hq, p.cache.H);
   if (p.max_attn_len < 0 || p.contextual_seq_len < 0)

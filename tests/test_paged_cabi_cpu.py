@@ -70,6 +70,15 @@ def test_attention_into_an_address_of_no_vector(field):
     assert rc == -1 and b"aligned" in why
 
 
+@pytest.mark.parametrize("rows", [-1, 1 << 31, 1 << 62, (1 << 62) + 1])
+def test_numbers_of_rows_that_overflow(rows):
+    rc, why = call("b200_hstu_paged_attn_fwd", attn(rows=rows, Hq=4))
+    assert rc == -1 and b"rows" in why
+    lib = ctypes.CDLL(_cabi.LIB_PATH)
+    lib.b200_hstu_paged_attn_workspace_bytes.restype = I64
+    assert lib.b200_hstu_paged_attn_workspace_bytes(ctypes.byref(attn(rows=rows, Hq=4))) == 0
+
+
 @pytest.mark.parametrize("which", [0, 1])
 @pytest.mark.parametrize("backward", [False, True])
 def test_norm_and_rotation_into_an_address_of_no_vector(backward, which):
