@@ -200,13 +200,14 @@ __device__ __forceinline__ void leave_join(const PagedAttn &a, const Walk<RB, TI
   a.joins[2 * blockIdx.x] = make_int4(c1, min(RB, w.seq.rows - w.rb * RB), w.h, w.rb * RB);
   a.joins[2 * blockIdx.x + 1] = make_int4(w.seq.q_start, 0, 0, 0);
 }
-// rows of q that no sequence has: zeros
+// rows of q that no sequence has, before the first offset and past the last: zeros
 template <typename T, int D, int THREADS>
 __device__ __forceinline__ void clear_rows_of_nobody(const PagedAttn &a) {
-  const int64_t from = a.cache.B > 0 ? max(0, a.q_offsets[a.cache.B]) : 0, row = (int64_t)a.Hq * D;
-  for (int64_t x = from * row + (int64_t)blockIdx.x * THREADS + threadIdx.x; x < a.rows * row;
-       x += (int64_t)gridDim.x * THREADS)
-    static_cast<T *>(a.out)[x] = from_f32<T>(0.f);
+  const int64_t row = (int64_t)a.Hq * D;
+  const int64_t before = a.cache.B > 0 ? min((int64_t)max(0, a.q_offsets[0]), a.rows) * row : 0;
+  const int64_t from = a.cache.B > 0 ? max(0, a.q_offsets[a.cache.B]) * row : 0;
+  for (int64_t x = (int64_t)blockIdx.x * THREADS + threadIdx.x; x < before + a.rows * row - from; x += (int64_t)gridDim.x * THREADS)
+    static_cast<T *>(a.out)[x < before ? x : x - before + from] = from_f32<T>(0.f);
 }
 
 // ---------------------------------------------------------------------------------------

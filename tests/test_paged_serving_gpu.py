@@ -84,3 +84,23 @@ def test_fields_that_do_not_fit_any_more(field, value):
         G.read_paged_kv(cache, table, offsets_of([1]), 1)
     with pytest.raises((RuntimeError, TypeError)):
         G.paged_mha(16, 1.0, x, cache, table, one, offsets_of([1]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [1, 12, 40])
+def test_rows_before_the_first_offset_and_past_the_last(rows, dtype):
+    """Rows of q that no sequence has are zeros, on either side."""
+    cache = G.PagedKVCache(torch.full((4, 2, G.PagedKVCache.page_bytes(64, 64)), 0x3e, dtype=torch.uint8, device=DEV), 64, 64)
+    table = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device=DEV)
+    lengths, off = torch.tensor([100, 77], device=DEV), 5 + offsets_of([rows, rows])
+    q = torch.randn(5 + 2 * rows + 9, 4, 64, device=DEV).to(dtype)
+    for act in ("silu", "softmax"):
+        torch.full_like(q, float("nan"))   # (what the allocator hands out next)
+        out = G.paged_mha(128, 0.1, q, cache, table, lengths, off, activation=act)
+        same = G.paged_mha(128, 0.1, q[5:5 + 2 * rows], cache, table, lengths, off - 5, activation=act)
+        assert float(out[:5].abs().sum()) == 0 and float(out[5 + 2 * rows:].abs().sum()) == 0
+        assert torch.isfinite(same).all()
+        assert float((out[5:5 + 2 * rows] - same).float().norm()) <= (2.0 ** -7 if dtype == torch.bfloat16 else 1e-5) * float(same.float().norm())
+    none = G.paged_mha(128, 0.1, q, cache, table[:0], lengths[:0], torch.zeros(1, dtype=torch.long, device=DEV))
+    assert float(none.abs().sum()) == 0
