@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(PC_THREADS, 3) paged_append_kernel(Append a) {
           }
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            if (e0 + i < rot.rotary) f[i] = __fadd_rn(__fmul_rn(f[i], c[i]), __fmul_rn(t[i], s[i]));
+            f[i] = e0 + i < rot.rotary ? __fadd_rn(__fmul_rn(f[i], c[i]), __fmul_rn(t[i], s[i])) : __fmul_rn(f[i], c[i]);
         }
       }
       const float top = group_top(f, mates);

@@ -222,6 +222,8 @@ __global__ void __launch_bounds__(NR_THREADS) norm_rotary_any_kernel(NormRotary 
         const float c = in ? a.rot.cos[pos * (a.rot.rotary >> 1) + k] : nan;
         const float s = (in ? a.rot.sin[pos * (a.rot.rotary >> 1) + k] : nan) * (leads(e, a.rot) ? -back : back);
         f = f * c + value(partner_of(e, a.rot)) * s;
+      } else if (rotate && !in) {
+        f = nan;
       }
       return f;
     };

@@ -83,7 +83,7 @@ __device__ __forceinline__ bool leads(int e, const Rotation &r) {
 }
 
 // Cosines, and sines with the sign that they have in `own * c + partner * s`, of a lane's eight values;
-// positions outside the tables give NaN.  VEC: rotary is a multiple of 16 and the tables are 16-byte aligned.
+// positions outside the tables give NaN, as cosines of values that are not rotated too.  VEC: rotary is a multiple of 16 and the tables are 16-byte aligned.
 template <bool VEC>
 __device__ __forceinline__ void angles8(const Rotation &r, int64_t pos, int e0, float (&c)[8], float (&s)[8]) {
   const bool in = pos >= 0 && pos < r.table_rows;
@@ -115,7 +115,7 @@ __device__ __forceinline__ void angles8(const Rotation &r, int64_t pos, int e0, 
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int e = e0 + i;
-    c[i] = 1.f, s[i] = 0.f;
+    c[i] = in ? 1.f : nan, s[i] = 0.f;
     if (e < r.rotary) {
       const int k = angle_of(e, r);
       c[i] = in ? r.cos[row + k] : nan;

@@ -104,3 +104,30 @@ def test_rows_before_the_first_offset_and_past_the_last(rows, dtype):
         assert float((out[5:5 + 2 * rows] - same).float().norm()) <= (2.0 ** -7 if dtype == torch.bfloat16 else 1e-5) * float(same.float().norm())
     none = G.paged_mha(128, 0.1, q, cache, table[:0], lengths[:0], torch.zeros(1, dtype=torch.long, device=DEV))
     assert float(none.abs().sum()) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("d,rotary", [(64, 32), (128, 64), (128, 20), (256, 64), (96, 32), (64, 64)])
+def test_positions_outside_the_tables_with_a_part_rotated(d, rotary, interleaved):
+    """The whole row is NaN, also what is not rotated; with and without a norm, forward and backward."""
+    cos, sin = G.rotary_tables(16, rotary, device=DEV)
+    pos = torch.tensor([0, 15, 16, -1, 3], device=DEV)
+    bad = torch.tensor([False, False, True, True, False])
+    for weight in (None, torch.ones(d, device=DEV)):
+        for dtype in (torch.float32, torch.bfloat16):
+            x = torch.randn(5, 2, d, device=DEV).to(dtype).requires_grad_()
+            y = G.qk_norm_rotary(x, None, pos, cos, sin, weight, interleaved=interleaved)[0]
+            (dx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+            for t in (y.detach(), dx):
+                nan = torch.isnan(t).flatten(1).cpu()
+                assert torch.equal(nan.all(1), bad) and torch.equal(nan.any(1), bad)
+            if d in G.paged_cache.HEAD_DIMS:
+                cache = G.PagedKVCache.allocate(2, 2, d, 16)
+                table = torch.tensor([[0, 1]], dtype=torch.int32, device=DEV)
+                k = x.detach()
+                G.append_paged_kv(cache, k, k, table, torch.tensor([14], device=DEV), offsets_of([5]), cos, sin, interleaved, weight)
+                both = G.read_paged_kv(cache, table, offsets_of([19]), 19)
+                nan = torch.isnan(both[0][14:]).flatten(1).cpu()
+                want = torch.tensor([False, False, True, True, True])
+                assert torch.equal(nan.all(1), want) and torch.equal(nan.any(1), want) and torch.isfinite(both[1][14:]).all()
