@@ -383,14 +383,11 @@ int norm_rotary(const b200_hstu_norm_rotary_args &p, bool bwd, cudaStream_t st) 
       return fail(B200_HSTU_EINVAL, "norm_rotary: results must be 16-byte aligned");
     if (bwd && a.w[i] && !p.dweight[i]) return fail(B200_HSTU_EINVAL, "norm_rotary: null tensor");
   }
-  if (p.H[0] + p.H[1] == 0) return 0;
-  if (p.rows == 0) {
-    for (int i = 0; bwd && i < 2; ++i) {
-      if (!a.w[i]) continue;
-      if (int rc = check_cuda(cudaMemsetAsync(p.dweight[i], 0, p.d * sizeof(float), st), "cudaMemsetAsync")) return rc;
-    }
-    return 0;
+  for (int i = 0; bwd && i < 2; ++i) {   // a sum over nothing
+    if (!p.weight[i] || !p.dweight[i] || (p.rows > 0 && p.H[i] > 0)) continue;
+    if (int rc = check_cuda(cudaMemsetAsync(p.dweight[i], 0, p.d * sizeof(float), st), "cudaMemsetAsync")) return rc;
   }
+  if (p.rows == 0 || p.H[0] + p.H[1] == 0) return 0;
   if (bwd && (a.w[0] || a.w[1])) {
     a.partial = static_cast<float *>(p.workspace);
     if (!p.workspace || p.workspace_bytes < norm_rotary_bwd_workspace_bytes(p.d))

@@ -131,3 +131,18 @@ def test_positions_outside_the_tables_with_a_part_rotated(d, rotary, interleaved
                 nan = torch.isnan(both[0][14:]).flatten(1).cpu()
                 want = torch.tensor([False, False, True, True, True])
                 assert torch.equal(nan.all(1), want) and torch.equal(nan.any(1), want) and torch.isfinite(both[1][14:]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q_heads,k_heads", [(0, 0), (0, 3), (3, 0)])
+def test_gradients_of_the_weights_of_no_heads(q_heads, k_heads):
+    w = [torch.ones(64, device=DEV, requires_grad=True) for _ in range(2)]
+    q, k = (torch.randn(5, h, 64, device=DEV, requires_grad=True) for h in (q_heads, k_heads))
+    for _ in range(3):
+        out = G.qk_norm_rotary(q, k, q_weight=w[0], k_weight=w[1])
+        dy = tuple(torch.ones_like(t) for t in out)
+        poison = [torch.full((64,), float("nan"), device=DEV) for _ in range(8)]   # (what the allocator hands out next)
+        del poison
+        dw = torch.autograd.grad(out, w, dy)
+        for grad, heads in zip(dw, (q_heads, k_heads)):
+            assert torch.isfinite(grad).all() and (float(grad.abs().sum()) == 0) == (heads == 0)
