@@ -73,6 +73,10 @@ class RotarySTULayer(STULayer):
                 uvqk_weight=as_dtype(self._uvqk_weight, x.dtype), uvqk_bias=as_dtype(self._uvqk_beta, x.dtype),
                 kernel=self._hammer_kernel)
 
+    def _head_weight(self, w, like):
+        # (q and k may be of another type than the parameters, as under autocast; the kernels take fp32 or theirs)
+        return w if w.dtype == like.dtype else as_dtype(w, torch.float32)
+
     def _output(self, attn, u, x):
         with span("## stu_compute_output ##"):
             return hstu_compute_output(
@@ -95,7 +99,7 @@ class RotarySTULayer(STULayer):
         with span("## qk_norm_rotary ##"):
             q, k = qk_norm_rotary(q.view(-1, self._num_heads, self._attention_dim),
                                   k.view(-1, self._num_heads, self._attention_dim), positions, self._cos, self._sin,
-                                  self._q_norm_weight, self._k_norm_weight)
+                                  self._head_weight(self._q_norm_weight, q), self._head_weight(self._k_norm_weight, k))
         with span("## hstu_mha ##"):
             attn = hstu_mha(max_seq_len=max_seq_len, alpha=self._attn_alpha, q=q, k=k,
                             v=v.view(-1, self._num_heads, self._hidden_dim), seq_offsets=x_offsets, causal=self._causal,
@@ -127,10 +131,11 @@ class RotarySTULayer(STULayer):
         lengths = cached_lengths + (new_offsets[1:] - new_offsets[:-1]).to(cached_lengths.dtype)
         positions = _new_positions(cached_lengths, new_offsets, new_x.shape[0])
         with span("## qk_norm_rotary ##"):
-            q, _ = qk_norm_rotary(q.view(-1, H, d), None, positions, self._cos, self._sin, self._q_norm_weight)
+            q, _ = qk_norm_rotary(q.view(-1, H, d), None, positions, self._cos, self._sin,
+                                  self._head_weight(self._q_norm_weight, q))
         with span("## append_paged_kv ##"):
             append_paged_kv(cache, k.view(-1, H, d), v.view(-1, H, d), page_table, cached_lengths, new_offsets, self._cos,
-                            self._sin, k_weight=self._k_norm_weight)
+                            self._sin, k_weight=self._head_weight(self._k_norm_weight, k))
         with span("## paged_mha ##"):
             attn = paged_mha(max_seq_len, self._attn_alpha, q, cache, page_table, lengths, new_offsets,
                              num_targets if self._target_aware else None, self._max_attn_len, self._contextual_seq_len,

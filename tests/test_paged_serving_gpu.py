@@ -146,3 +146,31 @@ def test_gradients_of_the_weights_of_no_heads(q_heads, k_heads):
         dw = torch.autograd.grad(out, w, dy)
         for grad, heads in zip(dw, (q_heads, k_heads)):
             assert torch.isfinite(grad).all() and (float(grad.abs().sum()) == 0) == (heads == 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("autocast", [None, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("params", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [torch.float32, torch.bfloat16, torch.float16])
+def test_rows_of_another_type_than_the_parameters(rows, params, autocast):
+    """What ``STULayer`` takes and gives, in training and served."""
+    layer = layer_of(params)
+    plain = G.STULayer(G.STULayerConfig(embedding_dim=96, num_heads=2, hidden_dim=64, attention_dim=64, output_dropout_ratio=0.0))
+    plain = plain.to(DEV).to(params).eval()
+    x = torch.randn(50, 96, device=DEV).to(rows)
+    off = offsets_of([20, 30])
+    with torch.autocast("cuda", autocast or torch.bfloat16, enabled=autocast is not None):
+        outs = []
+        for m in (plain, layer):
+            leaf = x.clone().requires_grad_()
+            outs.append(m(leaf, off[1:] - off[:-1], off, 64, None))
+            outs[-1].float().square().mean().backward()
+            assert leaf.grad.dtype == rows and torch.isfinite(leaf.grad).all()
+        cache = layer.new_cache(4, 64)
+        served = layer.paged_forward(x, cache, torch.arange(4, dtype=torch.int32, device=DEV).view(2, 2),
+                                     torch.zeros(2, dtype=torch.long, device=DEV), off, 64)
+    for p in layer.parameters():
+        assert p.grad is not None and p.grad.dtype == params and torch.isfinite(p.grad).all()
+    assert outs[0].dtype == outs[1].dtype == served.dtype
+    # (the served rows go through 4 bits)
+    assert float((served.float() - outs[1].float()).norm()) <= 0.25 * float(outs[1].float().norm())
