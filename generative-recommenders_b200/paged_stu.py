@@ -108,6 +108,9 @@ class RotarySTULayer(STULayer):
                             kernel=self._hammer_kernel)
         return self._output(attn, u, x)
 
+    def cached_forward(self, delta_x, num_targets, max_kv_caching_len=0, kv_caching_lengths=None):
+        raise NotImplementedError("RotarySTULayer serves from a paged cache: paged_forward")
+
     @torch.no_grad()
     def paged_forward(
         self,

@@ -174,3 +174,11 @@ def test_rows_of_another_type_than_the_parameters(rows, params, autocast):
     assert outs[0].dtype == outs[1].dtype == served.dtype
     # (the served rows go through 4 bits)
     assert float((served.float() - outs[1].float()).norm()) <= 0.25 * float(outs[1].float().norm())
+
+
+def test_the_16_bit_cache_is_not_served_from():
+    layer = G.RotarySTULayer(G.RotarySTULayerConfig(embedding_dim=8, num_heads=1, hidden_dim=64, attention_dim=64))
+    with pytest.raises(NotImplementedError, match="paged_forward"):
+        layer.cached_forward(torch.zeros(2, 8), None)
+    with pytest.raises(NotImplementedError, match="paged_forward"):
+        G.STUStack([layer]).cached_forward(torch.zeros(2, 8), None)
