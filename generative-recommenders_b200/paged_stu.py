@@ -129,6 +129,7 @@ class RotarySTULayer(STULayer):
         the layer was trained with.  Candidates (``num_targets``) that are not to stay are overwritten by the next
         call when it is given the same ``cached_lengths``.  Rows past ``new_offsets[-1]`` (padding) are in no sequence:
         nothing is cached for them and their attention is zeros."""
+        torch._assert(self._causal, "only support causal attention")
         H, d = self._num_heads, self._attention_dim
         u, q, k, v = self._uqvk(new_x)
         lengths = cached_lengths + (new_offsets[1:] - new_offsets[:-1]).to(cached_lengths.dtype)

@@ -182,3 +182,9 @@ def test_the_16_bit_cache_is_not_served_from():
         layer.cached_forward(torch.zeros(2, 8), None)
     with pytest.raises(NotImplementedError, match="paged_forward"):
         G.STUStack([layer]).cached_forward(torch.zeros(2, 8), None)
+
+
+def test_only_causal_layers_are_served():
+    layer = G.RotarySTULayer(G.RotarySTULayerConfig(embedding_dim=8, num_heads=1, hidden_dim=64, attention_dim=64, causal=False))
+    with pytest.raises(AssertionError, match="causal"):
+        layer.paged_forward(torch.zeros(2, 8), None, None, torch.zeros(1, dtype=torch.long), offsets_of([2], "cpu"), 8)
