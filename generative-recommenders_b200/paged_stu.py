@@ -99,7 +99,8 @@ class RotarySTULayer(STULayer):
         with span("## qk_norm_rotary ##"):
             q, k = qk_norm_rotary(q.view(-1, self._num_heads, self._attention_dim),
                                   k.view(-1, self._num_heads, self._attention_dim), positions, self._cos, self._sin,
-                                  self._head_weight(self._q_norm_weight, q), self._head_weight(self._k_norm_weight, k))
+                                  self._head_weight(self._q_norm_weight, q), self._head_weight(self._k_norm_weight, k),
+                                  kernel=self._hammer_kernel)
         with span("## hstu_mha ##"):
             attn = hstu_mha(max_seq_len=max_seq_len, alpha=self._attn_alpha, q=q, k=k,
                             v=v.view(-1, self._num_heads, self._hidden_dim), seq_offsets=x_offsets, causal=self._causal,
@@ -136,10 +137,10 @@ class RotarySTULayer(STULayer):
         positions = _new_positions(cached_lengths, new_offsets, new_x.shape[0])
         with span("## qk_norm_rotary ##"):
             q, _ = qk_norm_rotary(q.view(-1, H, d), None, positions, self._cos, self._sin,
-                                  self._head_weight(self._q_norm_weight, q))
+                                  self._head_weight(self._q_norm_weight, q), kernel=self._hammer_kernel)
         with span("## append_paged_kv ##"):
             append_paged_kv(cache, k.view(-1, H, d), v.view(-1, H, d), page_table, cached_lengths, new_offsets, self._cos,
-                            self._sin, k_weight=self._head_weight(self._k_norm_weight, k))
+                            self._sin, k_weight=self._head_weight(self._k_norm_weight, k), kernel=self._hammer_kernel)
         with span("## paged_mha ##"):
             attn = paged_mha(max_seq_len, self._attn_alpha, q, cache, page_table, lengths, new_offsets,
                              num_targets if self._target_aware else None, self._max_attn_len, self._contextual_seq_len,

@@ -188,3 +188,28 @@ def test_only_causal_layers_are_served():
     layer = G.RotarySTULayer(G.RotarySTULayerConfig(embedding_dim=8, num_heads=1, hidden_dim=64, attention_dim=64, causal=False))
     with pytest.raises(AssertionError, match="causal"):
         layer.paged_forward(torch.zeros(2, 8), None, None, torch.zeros(1, dtype=torch.long), offsets_of([2], "cpu"), 8)
+
+
+def test_every_operator_is_told_the_kernel(monkeypatch):
+    layer = G.RotarySTULayer(G.RotarySTULayerConfig(embedding_dim=8, num_heads=1, hidden_dim=64, attention_dim=64, max_positions=9))
+    layer._hammer_kernel = object()
+    told = {}
+
+    def fake(name, result):
+        def op(*args, kernel=None, **kwargs):
+            told[name] = kernel
+            return result
+        monkeypatch.setattr(paged_stu, name, op)
+
+    x = torch.zeros(2, 1, 64)
+    fake("hstu_compute_uvqk", (x, x, x, x))
+    fake("qk_norm_rotary", (x, x))
+    fake("append_paged_kv", None)
+    fake("paged_mha", x)
+    fake("hstu_mha", x)
+    fake("hstu_compute_output", x)
+    layer.paged_forward(torch.zeros(2, 8), None, None, torch.zeros(1, dtype=torch.long), offsets_of([2], "cpu"), 8)
+    assert len(told) == 5 and all(kernel is layer._hammer_kernel for kernel in told.values())
+    told.clear()
+    layer(torch.zeros(2, 8), torch.tensor([2]), offsets_of([2], "cpu"), 8, None)
+    assert len(told) == 4 and all(kernel is layer._hammer_kernel for kernel in told.values())
