@@ -202,7 +202,7 @@ def test_every_operator_is_told_the_kernel(monkeypatch):
         monkeypatch.setattr(paged_stu, name, op)
 
     x = torch.zeros(2, 1, 64)
-    fake("hstu_compute_uvqk", (x, x, x, x))
+    fake("hstu_compute_uqvk", (x, x, x, x))
     fake("qk_norm_rotary", (x, x))
     fake("append_paged_kv", None)
     fake("paged_mha", x)
