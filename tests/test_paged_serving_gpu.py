@@ -5,6 +5,7 @@ import torch
 
 import generative_recommenders_b200 as G
 from generative_recommenders_b200 import paged_stu
+from oracle import paged_oracle as P
 
 DEV = "cuda:0"
 
@@ -213,3 +214,48 @@ def test_every_operator_is_told_the_kernel(monkeypatch):
     told.clear()
     layer(torch.zeros(2, 8), torch.tensor([2]), offsets_of([2], "cpu"), 8, None)
     assert len(told) == 4 and all(kernel is layer._hammer_kernel for kernel in told.values())
+
+
+FEW = [([600], [1]), ([900, 300], [1, 1]), ([500, 200], [8, 5]), ([400, 30], [16, 12])]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("softmax", [False, True])
+@pytest.mark.parametrize("lengths,new", FEW)
+def test_weights_of_few_rows_keep_sixteen_bits(lengths, new, softmax):
+    """The kernel for few rows rounds weights to the sum of two bfloat16 numbers.  float16 results, element by element: 2^-16 of
+    every weight, 2^-16 of the sizes that a score is the sum of (codes stand 1024 above themselves in the product), half a
+    unit of the result."""
+    d, H = 128, 2
+    g = torch.Generator().manual_seed(5)
+    need = [-(-n // 64) for n in lengths]
+    pool = torch.randint(0, 256, (sum(need), H, G.PagedKVCache.page_bytes(64, d)), generator=g).to(torch.uint8)
+    codes = pool[..., :64 * d]
+    codes.copy_(torch.where(codes & 15 == 0, codes | 8, codes))
+    codes.copy_(torch.where(codes >> 4 == 0, codes | 128, codes))
+    scales = (torch.rand(sum(need), H, 2 * 64 * d // 64, generator=g) * 0.3 + 0.2).bfloat16()
+    pool[..., 64 * d:] = scales.view(torch.uint8)
+    cache = G.PagedKVCache(pool.to(DEV), 64, d)
+    table = torch.full((len(lengths), max(need)), -1, dtype=torch.int32)
+    for b, n in enumerate(need):
+        table[b, :n] = torch.arange(n) + sum(need[:b])
+    q = torch.randn(sum(new), 4, d, generator=g).half().to(DEV)
+    got = G.paged_mha(1, d ** -0.5, q, cache, table.to(DEV), torch.tensor(lengths, device=DEV), offsets_of(new),
+                      activation="softmax" if softmax else "silu", attn_scale=0.02).double()
+    at = 0
+    for b, (n, m) in enumerate(zip(lengths, new)):
+        k, v = (x.to(DEV).repeat_interleave(2, 1).transpose(0, 1) for x in P.read_rows(cache, table[b], n)[:2])
+        x = q[at:at + m].double().transpose(0, 1)
+        s, off = x @ k.transpose(1, 2) * d ** -0.5, 2.0 ** -16 * (x.abs() @ k.abs().transpose(1, 2)) * d ** -0.5
+        seen = torch.arange(n, device=DEV)[None] <= torch.arange(n - m, n, device=DEV)[:, None]
+        none = torch.zeros((), dtype=torch.float64, device=DEV)
+        if softmax:
+            w = torch.softmax(s.masked_fill(~seen, float("-inf")), -1)
+            error, common = w * (2.0 ** -16 + off), (w * off).sum(-1, keepdim=True) + 2.0 ** -20
+        else:
+            w = torch.where(seen, s * torch.sigmoid(s) * 0.02, none)
+            error, common = torch.where(seen, 2.0 ** -16 * w.abs() + 1.1 * 0.02 * off, none), 2.0 ** -20
+        out = w @ v
+        bound = error @ v.abs() + out.abs() * (common + 2.0 ** -11) + 2.0 ** -25
+        at += m
+        assert bool(((got[at - m:at].transpose(0, 1) - out).abs() <= bound).all())
