@@ -259,3 +259,40 @@ def test_weights_of_few_rows_keep_sixteen_bits(lengths, new, softmax):
         bound = error @ v.abs() + out.abs() * (common + 2.0 ** -11) + 2.0 ** -25
         at += m
         assert bool(((got[at - m:at].transpose(0, 1) - out).abs() <= bound).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,width", [([1, 0, 1], 7), ([3, 1, 2], 100), ([40, 20, 7], 7), ([300, 20, 0], 100)])
+def test_a_captured_step_is_the_step(new, width):
+    """``paged_forward`` in a CUDA graph, replayed with other rows, lengths, offsets and pages."""
+    layer = layer_of(torch.bfloat16, max_attn_len=50)
+    rows = sum(new) + 3
+    caches = [G.PagedKVCache(torch.zeros(90, 2, G.PagedKVCache.page_bytes(16, 64), dtype=torch.uint8, device=DEV), 16, 64)
+              for _ in range(2)]
+    table = torch.full((3, width), -1, dtype=torch.int32, device=DEV)
+    x = torch.zeros(rows, 96, device=DEV, dtype=torch.bfloat16)
+    cached, off = torch.zeros(3, dtype=torch.long, device=DEV), torch.zeros(4, dtype=torch.long, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            layer.paged_forward(x, caches[0], table, cached, off, 200)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer.paged_forward(x, caches[0], table, cached, off, 200)
+    done = torch.zeros(3, dtype=torch.long)
+    g = torch.Generator().manual_seed(1)
+    pages = min(width, 30)
+    table[:, :pages] = torch.randperm(90, generator=g)[:3 * pages].view(3, pages).to(torch.int32).to(DEV)
+    for step in range(3):
+        n = torch.tensor(new).roll(step)
+        x.copy_(torch.randn(rows, 96, generator=g))
+        cached.copy_(done)
+        off.copy_(torch.cat([torch.zeros(1, dtype=torch.long), n.cumsum(0)]))
+        graph.replay()
+        want = layer.paged_forward(x, caches[1], table, cached, off, 200)
+        # (rows without a page, or past the rotation's tables, are NaN in both)
+        assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(out.nan_to_num(7.0), want.nan_to_num(7.0))
+        assert torch.equal(caches[0].pages, caches[1].pages)
+        done += n
