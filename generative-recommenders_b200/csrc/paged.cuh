@@ -16,7 +16,9 @@ struct PagedCache {
 
   __host__ __device__ __forceinline__ int page_size() const { return 1 << page_shift; }
   // positions that a sequence can have pages for
-  __device__ __forceinline__ int positions() const { return (int)min((int64_t)width << page_shift, (int64_t)0x7ffffc00); }
+  __device__ __forceinline__ int positions() const {
+    return (int)min((int64_t)width << page_shift, (int64_t)0x7ffffc00);
+  }
   __host__ __device__ __forceinline__ int code_bytes() const { return d >> 1; }                    // of a row
   __host__ __device__ __forceinline__ int scale_bytes() const { return 2 * (d / PAGED_GROUP); }    // of a row
   __host__ __device__ __forceinline__ int64_t page_bytes() const {

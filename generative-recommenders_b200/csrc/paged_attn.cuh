@@ -206,7 +206,8 @@ __device__ __forceinline__ void clear_rows_of_nobody(const PagedAttn &a) {
   const int64_t row = (int64_t)a.Hq * D;
   const int64_t before = a.cache.B > 0 ? min((int64_t)max(0, a.q_offsets[0]), a.rows) * row : 0;
   const int64_t from = a.cache.B > 0 ? max(0, a.q_offsets[a.cache.B]) * row : 0;
-  for (int64_t x = (int64_t)blockIdx.x * THREADS + threadIdx.x; x < before + a.rows * row - from; x += (int64_t)gridDim.x * THREADS)
+  for (int64_t x = (int64_t)blockIdx.x * THREADS + threadIdx.x; x < before + a.rows * row - from;
+       x += (int64_t)gridDim.x * THREADS)
     static_cast<T *>(a.out)[x < before ? x : x - before + from] = from_f32<T>(0.f);
 }
 
@@ -232,8 +233,8 @@ __device__ __forceinline__ uint32_t masked_or(uint32_t x) {
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "n"(MASK), "r"(BITS));
   return r;
 }
-// float16: a code in the low bits of 1024's mantissa is 1024 + code, four bits further up
-// 1024 + 16 code - pairs 0 and 1 of `x` without a shift, 2 and 3 of x >> 8.  Pair i holds codes i and i + 4.
+// float16: a code in the low bits of 1024's mantissa is 1024 + code (the usual way to a float without a conversion),
+// four bits further up 1024 + 16 code - pairs 0 and 1 of `x` without a shift, 2 and 3 of x >> 8.  Pair i holds codes i and i + 4.
 __device__ __forceinline__ uint32_t k_pair(uint32_t x, bool up) {
   return up ? masked_or<0x00f000f0u, 0x64006400u>(x) : masked_or<0x000f000fu, 0x64006400u>(x);
 }

@@ -13,22 +13,23 @@
 //                them up at its end; then q of the next unit is in shared memory already.
 //
 // Rounding: (code - 8) * scale has at most 11 significant bits, so in float16 it is exact for scales from 2^12 down to
-// 2^-13 (odd pairs of codes are 16 times too large and meet a sixteenth of the scale).  K's scales are divided by a power of two
-// for each tile that leaves the largest at 2^12, and goes into the scores' factor; V's by one that leaves it at 2^9 to
-// 2^12 and changes where a tile's scales leave that range (the results, in fp32, are multiplied by the difference).  So
-// scales down to 2^-25 and 2^-22 of a tile's largest are exact, whichever rows see that one and whichever group of 64
-// values it is in; smaller ones lose a bit for each power of two.  q is scaled by a
-// power of two for each row.  The weights are float16 too, so they are held at a size of their own: for softmax the
-// largest so far is at 2^7 to 2^15; for SiLU 2^15 is what no score can reach, |alpha| D max |q| times the tile's largest
-// code and scale, which is 2^7 or so times the usual ones.  So no finite score overflows, and weights keep their 11 bits
-// down to 2^-21 of the largest (2^-29 of SiLU's bound).  What is rounded is a weight, to 11 bits, and the result;
-// tanh.approx, as in the attention over 16-bit keys, is off by 2^-11 of half the score.
+// 2^-13 (odd pairs of codes are 16 times too large and meet a sixteenth of the scale).  K's scales are divided by a
+// power of two for each tile that leaves the largest at 2^12, and goes into the scores' factor; V's by one that leaves
+// it at 2^9 to 2^12 and changes where a tile's scales leave that range (the results, in fp32, are multiplied by the
+// difference).  So scales down to 2^-25 and 2^-22 of a tile's largest are exact, whichever rows see that one and
+// whichever group of 64 values it is in; smaller ones lose a bit for each power of two.  q is scaled by a power of two
+// for each row.  The weights are float16 too, so they are held at a size of their own: for softmax the largest so far
+// is at 2^7 to 2^15; for SiLU 2^15 is what no score can reach, |alpha| D max |q| times the tile's largest code and
+// scale, which is 2^7 or so times the usual ones.  So no finite score overflows, and weights keep their 11 bits down to
+// 2^-21 of the largest (2^-29 of SiLU's bound).  What is rounded is a weight, to 11 bits, and the result; tanh.approx,
+// as in the attention over 16-bit keys, is off by 2^-11 of half the score.
 //
 // A score costs one operation of the special-function unit (16 a clock and SM), 128 x 128 of them 1024 clocks; the
-// tile's two products take 512 clocks at head dimension 128, the conversions about 500 issue slots of each
-// scheduler.  What bounds it is the row warps' way from scores to weights (some 3000 clocks for a tile and warp) and
-// the turns between them and the products.  Measured at head dimension 128: 256 rows for each of 32 histories of
-// 8192 450 TFLOP/s for SiLU and 329 for softmax; 128 users of 320 - 8192 with 256 candidates and 4 heads 455 us.
+// tile's two products take 512 clocks at head dimension 128.  Neither is the bound: special functions and products are
+// busy a third of the time each, and so are the issue slots.  What is, is the row warps' waiting for scores: 32 of them
+// are loaded from tensor memory, waited for and worked on, then the next 32, for softmax twice (the maximum first).
+// Measured at head dimension 128, 4 heads: 256 rows for each of 32 histories of 8192 221 us for SiLU (611 TFLOP/s) and
+// 241 us for softmax, 128 rows each 187 us; 128 users of 320 - 8192 with 256 candidates 422 - 464 us.
 #include "paged_attn.cuh"
 
 namespace b200hstu {
@@ -41,7 +42,7 @@ constexpr int TC_THREADS = 448, TC_WARPS = TC_THREADS / 32;
 constexpr int TC_ROWS = 128, TC_BLOCK = 2 * TC_ROWS, TC_TILE = 128;   // rows of a product, of a unit; positions of a tile
 constexpr int RING_SLOTS = 8;
 constexpr int RING_READERS = 13;  // 8 + 4 + 1 warps
-constexpr int SCALE_AT = 12;      // exponent of the largest scale that float16 has room for, code 0 too: 8 * 255 / 128 * 2^12 < 65504
+constexpr int SCALE_AT = 12;      // exponent of the largest scale that float16 has room for (code 0: 8 * 1.99 * 2^12 < 65504)
 enum { TILE_FIRST = 1, TILE_PAIR = 2, TILE_BAD = 4 };
 
 struct __align__(16) RingSlot {
@@ -526,7 +527,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
       }();
       float top = SOFTMAX ? -3.0e38f : 0.f, sum = 0.f;
       int ref = 0;          // the result so far is in units of 2^ref
-      uint32_t lost = sees.past(a.cache.positions()) ? 3 : 0;   // groups of 64 values in which the row sees a V that is no number
+      // groups of 64 values in which the row sees a V that is no number
+      uint32_t lost = sees.past(a.cache.positions()) ? 3 : 0;
       const uint32_t end = begin + here, before = count;
       const int first_pos = (walk.range.first_tile<TC_TILE>() + walk.tile) * TC_TILE;
       for (uint32_t i = begin; i < end && ok; ++i) {
@@ -540,7 +542,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attn_tc_kernel(PagedAttn 
         ok = ok && mbar_wait(wc, s_full + 8 * side, count & 1, 971);
         if (!ok) break;
         tc_fence_after();
-        const float factor = SOFTMAX ? fmaxf(mul * slot.k_factor, 1.2e-38f) : mul * slot.k_factor;   // (above 0: an unseen score stays -inf)
+        float factor = mul * slot.k_factor;
+        if (SOFTMAX) factor = fmaxf(factor, 1.2e-38f);   // (above 0: an unseen score stays -inf)
         const int v_exp = slot.v_exp;
         const int pos0 = first_pos + (int)(i - begin) * TC_TILE;
         const bool masked = pos0 < walk.range.all_lo || pos0 + TC_TILE > walk.range.all_hi;

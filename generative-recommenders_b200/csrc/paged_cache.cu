@@ -84,7 +84,8 @@ __device__ __forceinline__ uint32_t eight_codes(const float (&f)[8], float inver
 // of K or V of a row with one set of angles, neighbouring groups neighbouring rows.  The arithmetic is written with
 // explicit roundings (and the sum of squares neighbours first), so that a row has one set of codes whatever block it
 // falls into.
-// Bound by the instructions of rotating and rounding, not by bytes: 100 histories of 37 - 2001 rows of 8 heads of 64 in
+// Bound by the instructions of rotating and rounding, which are scalar (issue slots 62 %, DRAM 21 % of the time), not by
+// bytes: 100 histories of 37 - 2001 rows of 8 heads of 64 in
 // fp16 take 45 - 50 us (2.5 TB/s), 32 single rows 13 us with the call.  Four heads a group share a row's place and angles
 // (that history in 96 us with reading back, 140 with one head each); where rows are few, one head each: the single rows
 // 13.7 us, 16.8 with four.

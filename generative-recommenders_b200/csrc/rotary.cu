@@ -66,10 +66,12 @@ __device__ __forceinline__ float dot8(const float (&a)[8], const float (&b)[8]) 
 }
 
 // d = 8 * LANES.  blockIdx.y: q or k.  A group of LANES lanes takes NR_HEADS heads of one row; forward the weights meet
-// the angles once for all of them: y = rstd (x (w cos) + x' (w' sin)).  What limits it is how many loads are on their
-// way, so registers: a value's partner comes from its lane, as loaded, not by a load of its own.
-// Measured, bf16, 36865 rows of 4 + 4 heads of 128: forward 42 us (3.6 TB/s), backward 63 us (3.6 TB/s) and the sum of
-// dweight's parts 5 - 9 us; fp16, 200003 rows of 8 + 2 heads of 64: 127 and 195 us (4.0 TB/s).
+// the angles once for all of them: y = rstd (x (w cos) + x' (w' sin)).  A value's partner comes from its lane, as loaded,
+// not by a load of its own.  What limits it is that an item's loads, arithmetic and stores follow one another: warps wait
+// for loads most (issue slots 63 % forward, 53 % backward, DRAM 35 % and 44 % of the time), and no load of the next item
+// is under way meanwhile.
+// Measured, bf16, 36865 rows of 4 + 4 heads of 128: forward 39 - 42 us (3.6 TB/s), backward 56 - 63 us (3.6 TB/s) and the
+// sum of dweight's parts 5 - 9 us; fp16, 200003 rows of 8 + 2 heads of 64: 127 and 195 us (4.0 TB/s).
 template <typename T, int LANES, int MODE, bool VEC, bool BWD>
 __global__ void __launch_bounds__(NR_THREADS, nr_ctas(BWD)) norm_rotary_kernel(NormRotary a) {
   constexpr int D = 8 * LANES, GROUPS = NR_THREADS / LANES;

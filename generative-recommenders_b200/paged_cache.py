@@ -125,7 +125,13 @@ def paged_mha(
     A row that sees nothing gives zeros, one that sees a position without a page of the pool NaN; table entries
     that no row sees (those that a window has left behind) may hold anything.  The same call gives the same bits;
     where a long sequence's sums are cut depends on the work of the whole batch, so in another batch a row may differ
-    in the last of them.  No gradient: this is the inference path."""
+    in the last of them.  A group of V that is NaN makes that group's columns NaN of the rows that see it.  Rows of q before
+    the first offset and past the last are zeros.
+
+    Scores and sums are fp32.  Weights are rounded to 16 bits (float32 q: 24); from 17 rows a sequence of the batch on, with
+    16-bit q and heads of 64 or 128, to 11 bits, with SiLU's tanh off by 2^-11 of half the score as in
+    :func:`hstu_mha`'s 16-bit kernels.  Scales of any size are exact there down to 2^-22 of the largest of 128
+    positions' (smaller ones lose a bit for each power of two).  No gradient: this is the inference path."""
     _require_cuda_backend(kernel)
     torch._assert(max_seq_len > 0, "max_seq_len must be larger than 0")
     torch._assert(max_attn_len >= 0 and contextual_seq_len >= 0, "max_attn_len and contextual_seq_len must not be negative")

@@ -38,7 +38,10 @@ def _new_positions(cached_lengths: torch.Tensor, new_offsets: torch.Tensor, rows
 
 class RotarySTULayer(STULayer):
     """``STULayer`` with weights for the norms of q and k (``_q_norm_weight``, ``_k_norm_weight``, one entry per
-    value of a head) and rotated positions; ``attention_dim`` and ``hidden_dim`` are the same."""
+    value of a head) and rotated positions; ``attention_dim`` and ``hidden_dim`` are the same.
+
+    The projection, the norms and the attention are separate stages: ``recompute_uvqk`` and ``recompute_normed_x``, which
+    say what a fused one keeps for its backward, change nothing here, nor does ``sort_by_length``, which no kernel needs."""
 
     def __init__(self, config: RotarySTULayerConfig, is_inference: bool = False) -> None:
         if config.rel_bias_buckets > 0:

@@ -454,7 +454,8 @@ int b200_hstu_paged_read(const b200_hstu_paged_read_args *args, b200_hstu_stream
  * num_targets[b] positions see none of each other, max_attn_len > 0 limits the distance and contextual_seq_len
  * is the length of the contextual prefix.  A row that sees nothing is zero, one that sees a position without a
  * page of the pool (past the sequence's table, or on an entry that names none) NaN; entries that no row sees, such
- * as those that a window has left behind, may hold anything.
+ * as those that a window has left behind, may hold anything.  A scale of V that is no number makes its group's columns
+ * NaN of the rows that see it.  Rows of q before q_offsets[0] and past q_offsets[B] are zeros.
  */
 typedef struct b200_hstu_paged_attn_args {
   b200_hstu_paged_cache cache;
