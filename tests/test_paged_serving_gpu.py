@@ -224,8 +224,7 @@ FEW = [([600], [1]), ([900, 300], [1, 1]), ([500, 200], [8, 5]), ([400, 30], [16
 @pytest.mark.parametrize("lengths,new", FEW)
 def test_weights_of_few_rows_keep_sixteen_bits(lengths, new, softmax):
     """The kernel for few rows rounds weights to the sum of two bfloat16 numbers.  float16 results, element by element: 2^-16 of
-    every weight, 2^-16 of the sizes that a score is the sum of (codes stand 1024 above themselves in the product), half a
-    unit of the result."""
+    every weight, 2^-16 of the sizes that a score is the sum of, half a unit of the result."""
     d, H = 128, 2
     g = torch.Generator().manual_seed(5)
     need = [-(-n // 64) for n in lengths]
@@ -296,3 +295,28 @@ def test_a_captured_step_is_the_step(new, width):
         assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(out.nan_to_num(7.0), want.nan_to_num(7.0))
         assert torch.equal(caches[0].pages, caches[1].pages)
         done += n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 7])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_scores_of_few_rows_are_sums_in_32_bits(d, new):
+    """Rows that see one position: the result is SiLU of one score times V, in float16.  The score is a sum of terms of either
+    sign; what it may be off by goes with the terms' sizes: sums of up to twice those (odd codes stand 64 above themselves)
+    in four steps a group of 64, 2^-23 each, are 1.4e-6 of them; one rounding of the weight's 16 bits and of the result."""
+    B, H = 300, 4
+    g = torch.Generator().manual_seed(d + new)
+    pool = torch.randint(0, 256, (B, H, G.PagedKVCache.page_bytes(16, d)), generator=g).to(torch.uint8)
+    pool[..., 16 * d:] = (torch.rand(B, H, 2 * 16 * d // 64, generator=g) * 0.3 + 0.2).bfloat16().view(torch.uint8)
+    cache = G.PagedKVCache(pool.to(DEV), 16, d)
+    table = torch.arange(B, dtype=torch.int32)[:, None]
+    q = torch.randn(B * new, H, d, generator=g).half().to(DEV)
+    # candidates at the start of a sequence see themselves alone
+    many = torch.full((B,), new, device=DEV)
+    got = G.paged_mha(1, d ** -0.5, q, cache, table.to(DEV), many, offsets_of([new] * B), many, attn_scale=1.0).double()
+    rows = [P.read_rows(cache, table[b], new)[:2] for b in range(B)]
+    k, v = (torch.cat(x).to(DEV) for x in zip(*rows))
+    s, sizes = (q.double() * k).sum(-1, keepdim=True) * d ** -0.5, (q.double() * k).abs().sum(-1, keepdim=True) * d ** -0.5
+    w = s * torch.sigmoid(s)
+    bound = (2.0 ** -16 * w.abs() + 1.1 * 1.4e-6 * sizes) * v.abs() + 2.0 ** -11 * (w * v).abs() + 2.0 ** -25
+    assert float(((got - w * v).abs() / bound).max()) <= 1
