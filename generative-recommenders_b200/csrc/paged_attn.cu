@@ -99,12 +99,12 @@ template <> struct Terms<float> { static constexpr int Q = 3, P = 3; };
 // of its keys whatever column it stands for, and the four lanes that share keys take a block of the tile each: a
 // score's scales, mask, exponential and weight are worked out once, not eight times.
 //
-// What bounds it where there is work enough is not the bytes (46 % of DRAM's time) but short dependent chains at 2.7
-// warps a scheduler, with the pipe of the logic operations, most of them codes to numbers, busy 53 % of the time and
-// issue slots 49 %; elsewhere the way to the first tile and the joining.
-// Measured with the call and the join, heads of 128, bf16: one row of each of 512 users, 0.50 GB of cache, 151 - 158 us
-// (3.2 TB/s); of 32 users of 16384 each 75 us (3.8 TB/s), with 8 rows each 94 us, with 16 131 us; a history of 200001
-// with four rows for each of 2 key heads 33 us (1.6 TB/s).
+// What bounds it where there is work enough is not the bytes (47 % of DRAM's time) but short dependent chains at 2.7
+// warps a scheduler, with the pipe of the logic operations, most of them codes to numbers, busy 52 % of the time and
+// issue slots 51 %; elsewhere the way to the first tile and the joining.
+// Measured with the call and the join, heads of 128, bf16: one row of each of 512 users, 0.50 GB of cache, 155 - 160 us
+// (3.2 TB/s); of 32 users of 16384 each 77 us (3.7 TB/s), with 8 rows each 96 us, with 16 134 us; a history of 200001
+// with four rows for each of 2 key heads 34 us (1.6 TB/s).
 template <typename T, int D, int NT, bool SOFTMAX>
 __global__ void __launch_bounds__(PA_THREADS) paged_attn_kernel(PagedAttn a) {
   constexpr bool ONE = NT == 0;
@@ -709,7 +709,7 @@ constexpr int SMS = 148;
 constexpr int PA_MAX_CTAS = SMS * 5;
 constexpr int PA_MIN_TILES = 2;   // of a CTA, where the cache may be that long
 // Positions of a sequence that a CTA does by itself at most, by the width of the table: the lengths are on the device, so
-// short sequences under a wide table are cut and joined.  (4 users of up to 700: 10.6 us, 12 when cut and joined; 32
+// short sequences under a wide table are cut and joined.  (4 users of up to 700: 10.4 us, 12 when cut and joined; 32
 // users of up to 1024 with 20 rows each: 28.7 us and 43.)
 constexpr int WHOLE_UP_TO = 1024;
 
