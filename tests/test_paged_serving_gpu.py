@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import generative_recommenders_b200 as G
-from generative_recommenders_b200 import paged_stu
+from generative_recommenders_b200 import hstu_attention, paged_stu
 from oracle import paged_oracle as P
 
 DEV = "cuda:0"
@@ -262,8 +262,9 @@ def test_weights_of_few_rows_keep_sixteen_bits(lengths, new, softmax):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("new,width", [([1, 0, 1], 7), ([3, 1, 2], 100), ([40, 20, 7], 7), ([300, 20, 0], 100)])
-def test_a_captured_step_is_the_step(new, width):
+def test_a_captured_step_is_the_step(new, width, monkeypatch):
     """``paged_forward`` in a CUDA graph, replayed with other rows, lengths, offsets and pages."""
+    monkeypatch.setattr(hstu_attention, "_CHECK_STATUS", False)   # (which waits for every call)
     layer = layer_of(torch.bfloat16, max_attn_len=50)
     rows = sum(new) + 3
     caches = [G.PagedKVCache(torch.zeros(90, 2, G.PagedKVCache.page_bytes(16, 64), dtype=torch.uint8, device=DEV), 16, 64)
